@@ -116,6 +116,25 @@ _SIGNATURES = {
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
          c_int, c_void_p, c_int, c_void_p, c_size_t, c_void_p],
     ),
+    "axm_rope_paged_kv_write": (
+        c_int,
+        [c_void_p, c_int64, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p],
+    ),
+    "axm_paged_decode_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "axm_paged_flash_decode": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_size_t, c_void_p],
+    ),
+    "axm_evict_paged_kv": (
+        c_int,
+        [c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p,
+         c_void_p],
+    ),
+    "axm_sample_rows": (
+        c_int,
+        [c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_int,
+         c_float, c_float, c_void_p, c_void_p, c_void_p],
+    ),
     "axm_runner_create": (c_int, [c_void_p, c_void_p]),
     "axm_runner_destroy": (None, [c_void_p]),
     "axm_runner_step": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_void_p]),
@@ -165,6 +184,17 @@ class RunnerDesc(ctypes.Structure):
         ("k_scales", ctypes.POINTER(c_void_p)), ("v_scales", ctypes.POINTER(c_void_p)),
         ("max_tokens", c_int), ("layout", c_int), ("group_size", c_int),
         ("qkv_format", c_int), ("o_format", c_int), ("gu_format", c_int), ("down_format", c_int),
+    ]
+
+
+class PagedKv(ctypes.Structure):
+    """Mirror of axm_paged_kv (include/axm.h)."""
+
+    _fields_ = [
+        ("k", c_void_p), ("v", c_void_p), ("k_scales", c_void_p), ("v_scales", c_void_p), ("block_table", c_void_p),
+        ("page_stride", c_int64), ("scale_stride", c_int64),
+        ("kv_dtype", c_int), ("n_kv_head", c_int), ("head_dim", c_int), ("page_size", c_int), ("n_pages", c_int),
+        ("n_seqs", c_int), ("max_pages", c_int),
     ]
 
 

@@ -18,7 +18,13 @@ from .ops import (  # noqa: F401
     rope_kv_cache_write,
     rope_kv_cache_write_quantized,
     rope_tree_kv_cache_write,
+    sample_tokens,
     swiglu_gate_up,
+)
+from .paged import (  # noqa: F401
+    evict_paged_kv,
+    gqa_paged_decode,
+    rope_paged_kv_cache_write,
 )
 from .quant import (  # noqa: F401
     compute_quantization_metrics,

@@ -1,5 +1,5 @@
 """Decode-path operators (MI355X): KV quantization, split-KV decode attention,
-bitmask tree attention, RMSNorm / SwiGLU / argmax.
+bitmask tree attention, RMSNorm / SwiGLU / argmax, sampling.
 
 Mirrors the names and argument meaning of ``axiomlm.kernels.ops`` and the KV
 helpers of ``axiomlm.kernels.quant`` (axiomlm/kernels/ops.py:552-797,
@@ -8,6 +8,7 @@ axiomlm/kernels/quant.py:692-1008).  All compute runs in libaxm.so.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -22,6 +23,13 @@ def _kv_code(kv_dtype: str) -> int:
         return KV_CODES[kv_dtype.lower()]
     except KeyError:
         raise ValueError(f"unsupported kv_dtype {kv_dtype!r}") from None
+
+
+def on_device(device: torch.device):
+    """Makes the tensors' device the current one, for launches on its stream."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def _check_head_dim(head_dim: int, who: str) -> None:
@@ -342,3 +350,61 @@ def argmax_last_token(logits: torch.Tensor) -> torch.Tensor:
     _lib.check(_lib.lib().axm_argmax(_lib.ptr(logits.to(torch.float16).contiguous()), rows, V, _lib.ptr(out),
                                      _lib.stream_of(logits.device)), "argmax_last_token")
     return out
+
+
+_LOGIT_CODES = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 2}
+
+
+def _setting(who: str, name: str, x, dtype: torch.dtype, rows: int, device, low: float, high: float):
+    """A sampling setting of every row: (device array or None, value)."""
+    if isinstance(x, torch.Tensor) and x.dim() > 0:
+        if x.device != device or x.numel() != rows:
+            raise ValueError(f"{who}: {name} must have one entry per row ({rows}) on {device}, got {tuple(x.shape)} on "
+                             f"{x.device}")
+        return x.to(dtype).contiguous(), 0
+    x = x.item() if isinstance(x, torch.Tensor) else x
+    if not low <= x <= high:
+        raise ValueError(f"{who}: {name}={x} outside [{low}, {high}]")
+    return None, x
+
+
+def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                  return_probs: bool = False):
+    """One token per row of logits (..., V) (fp16, fp32 or bf16; rows may be strided), int64, from the given uniform
+    numbers (fp32 in [0, 1), one per row): ``argmax_last_token`` with randomness.
+
+    Each setting is a number or a tensor of one per row.  temperature divides the logits (0: the row's largest logit,
+    lowest index on ties); top_k (0: off) keeps the k largest; top_p (1: off) of those the shortest run, from the largest
+    down, that holds top_p of their probability; min_p (0: off) those at least min_p times as likely as the likeliest.
+    Equal logits: the lower index is kept first.  The token is the first kept one, in index order, at which the running
+    probability exceeds the uniform number.  -inf and NaN logits are never taken; +inf ones are taken alone.  A row with
+    nothing to take gives -1.  return_probs: also the token's probability among the kept, fp32."""
+    who = "sample_tokens"
+    _lib.require_gpu(logits, who)
+    if logits.dtype not in _LOGIT_CODES or logits.dim() < 1 or logits.size(-1) < 1:
+        raise ValueError(f"{who}: logits must be fp16, fp32 or bf16 (..., V), got {tuple(logits.shape)} {logits.dtype}")
+    V = logits.size(-1)
+    lead = logits.shape[:-1]
+    rows = logits.numel() // V
+    dev = logits.device
+    if not isinstance(uniforms, torch.Tensor) or uniforms.device != dev or uniforms.dtype != torch.float32 \
+            or uniforms.numel() != rows:
+        raise ValueError(f"{who}: uniforms must be fp32, one per row ({rows}) on {dev}")
+    inf = float("inf")
+    t, t_all = _setting(who, "temperature", temperature, torch.float32, rows, dev, 0.0, inf)
+    k, k_all = _setting(who, "top_k", top_k, torch.int32, rows, dev, 0, inf)
+    p, p_all = _setting(who, "top_p", top_p, torch.float32, rows, dev, 0.0, 1.0)
+    m, m_all = _setting(who, "min_p", min_p, torch.float32, rows, dev, 0.0, 1.0)
+    tokens = torch.empty(lead, dtype=torch.int64, device=dev)
+    probs = torch.empty(lead, dtype=torch.float32, device=dev) if return_probs else None
+    if rows:
+        z = logits.reshape(rows, V)
+        if z.stride(1) != 1 and V > 1 or rows > 1 and z.stride(0) < V:
+            z = z.contiguous()
+        u = uniforms.contiguous()
+        with on_device(dev):
+            _lib.check(_lib.lib().axm_sample_rows(
+                z.data_ptr(), _LOGIT_CODES[logits.dtype], z.stride(0) if rows > 1 else V, rows, V, u.data_ptr(),
+                _lib.ptr(t), _lib.ptr(k), _lib.ptr(p), _lib.ptr(m), float(t_all), min(int(k_all), V), float(p_all),
+                float(m_all), tokens.data_ptr(), _lib.ptr(probs), _lib.stream_of(dev)), who)
+    return (tokens, probs) if return_probs else tokens

@@ -261,6 +261,76 @@ int axm_gqa_tree_verify(const void* q, const void* k_cache, const void* v_cache,
                         int head_dim, int max_seq_len, int prefix_len, int write_pos, const void* masks_u64_dev,
                         int num_splits, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- paged KV cache: several sequences, each with its own pages and length ----------------- *
+ * No counterpart in the reference (its PagedKVCache, axiomlm/engine/paged_cache.py:4-120, gathers pages with
+ * tensor indexing and is deprecated).  A pool of n_pages pages holds the rows of all sequences: k and v
+ * [n_pages][Hkv][page_size][row], rows as in the contiguous caches above (fp16 / FP8 / INT4 codes with
+ * scales [n_pages][Hkv][page_size][hd/64]).  Slot s of sequence b is row s % page_size of page
+ * block_table[b][s / page_size].  Head size 64 or 128; page_size a power of two, 8 to 1024.  k, v and scale
+ * pages are 16-byte aligned (scales: 4-byte) and may be spaced further apart than dense ones.
+ * Tables, lengths and positions are read on the device, so captured graphs replay with new ones. */
+typedef struct axm_paged_kv {
+  void* k;
+  void* v;
+  void* k_scales; /* quantized caches only */
+  void* v_scales;
+  const int* block_table; /* device int32 [n_seqs][max_pages] */
+  int64_t page_stride;    /* bytes from a page of k (and of v) to the next */
+  int64_t scale_stride;   /* bytes from a page of scales to the next */
+  int kv_dtype, n_kv_head, head_dim, page_size, n_pages, n_seqs, max_pages;
+} axm_paged_kv;
+
+/* RoPE of T tokens' queries (in place) and keys, and their keys and values stored into the pages.  qkv fp16, token
+ * t's row of q_dim + 2 Hkv hd halves at qkv + t ld_qkv; qkv_bias fp16 or NULL; freqs fp32 [rope_len][hd/2][2].
+ * Token t (device int32 arrays of length T) belongs to sequence seq_ids[t] (t where seq_ids is NULL), is rotated at
+ * positions[t] modulo rope_len and stored at slot slots[t] (positions[t] where slots is NULL).  A token whose sequence,
+ * slot or page is out of range is padding: nothing of it is read or changed.  The key and value parts of qkv are left as
+ * they were.  No slot may be given twice in a call.  Rotation and codes as axm_rope_kv_cache_write, except that FP8
+ * codes saturate at 448 and a group whose scale rounds to zero has zero codes. */
+int axm_rope_paged_kv_write(void* qkv, int64_t ld_qkv, int T, const void* freqs, int rope_len, const int* positions,
+                            const int* slots, const int* seq_ids, const void* qkv_bias, const axm_paged_kv* kv,
+                            int q_dim, void* stream);
+
+/* Attention of one new token per sequence: q fp16 (sequence b's row of Hq hd halves at q + b ld_q, 16-byte aligned) ->
+ * out fp16 [n_seqs][Hq][hd], softmax(q k / sqrt(hd)) over slots [0, seq_lens[b]) (device int32, held to [0, max_pages
+ * page_size]); keys and values as axm_dequantize_kv gives them.  A sequence of length 0 gives zeros; keys on a page
+ * outside the pool are left out.  mass (or NULL): fp32 [n_seqs][Hkv][mass_len], mass_len >= max_pages page_size;
+ * the softmax weights of slot s, summed over the query heads of the KV head, are added to mass[b][kvh][s].
+ * workspace >= axm_paged_decode_workspace_bytes (256-byte aligned). */
+size_t axm_paged_decode_workspace_bytes(int n_seqs, int n_head, int n_kv_head, int head_dim, int page_size,
+                                        int max_pages, int with_mass);
+int axm_paged_flash_decode(const void* q, int64_t ld_q, const axm_paged_kv* kv, const int* seq_lens, void* out,
+                           int n_head, float* mass, int64_t mass_len, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
+/* Eviction by accumulated attention weight, all layers of a cache in one call: k and v of layer l start
+ * layer_stride bytes (scales: scale_layer_stride) after those of layer l - 1.  A sequence longer than budget keeps, per
+ * layer and KV head, its last `recent` slots and the budget - recent slots of largest mass before them (equal ones:
+ * the lower slot; NaN counts as less than every number); their rows move, in order, to slots 0 .. budget - 1 (the
+ * rows behind stay as they are).  mass fp32 [L][n_seqs][Hkv][mass_len] is read; mass_out (same shape, another buffer) has
+ * the kept slots' values and zeros behind them; kept int32 [L][n_seqs][Hkv][budget] the slots that the rows come from
+ * (-1 behind the last); lens_out int32 [n_seqs] = min(seq_lens, budget).  1 <= budget, 0 <= recent <= budget.  Pages
+ * of a sequence over the budget must not be shared with another one. */
+int axm_evict_paged_kv(const axm_paged_kv* kv, int n_layer, int64_t layer_stride, int64_t scale_layer_stride,
+                       const int* seq_lens, const float* mass, int64_t mass_len, int budget, int recent,
+                       float* mass_out, int* kept, int* lens_out, void* stream);
+
+/* ---- sampling ------------------------------------------------------------- *
+ * One token per row of logits [rows][V] (dtype 0: fp16, 1: fp32, 2: bf16; row r at logits + r ld elements), from the
+ * uniform numbers u fp32 [rows] in [0, 1).  Per row: w = exp((z - max z) / temperature); top_k (0: off) keeps the
+ * k largest logits (equal ones: the lower index); top_p (>= 1: off) of those the shortest prefix in the same order
+ * whose weight reaches top_p of theirs, one at least; min_p keeps w >= min_p.  The token is the first kept index, in
+ * index order, whose running sum of weights exceeds u times the kept ones' total.  temperature <= 0: the
+ * largest logit (the lower index).  Logits of -inf and NaN are never taken; where one is +inf only those count.  A row
+ * with nothing to take gives -1 (and probability 0).  Settings: a device array of one per row, or NULL and the
+ * value given.  probs fp32 [rows] or NULL: the token's share of the kept weights.  Sums are exact integers (weights are
+ * rounded to 46 bits below the largest, fewer from 131072 logits on), so results do not depend on the order of threads.
+ * The reference samples in Python (axiomlm/engine/inference.py); next to axm_argmax. */
+int axm_sample_rows(const void* logits, int dtype, int64_t ld, int rows, int V, const float* u,
+                    const float* temperature, const int* top_k, const float* top_p, const float* min_p,
+                    float temperature_all, int top_k_all, float top_p_all, float min_p_all, int64_t* tokens,
+                    float* probs, void* stream);
+
 /* ---- whole-model decode runner ------------------------------------------- *
  * Replaces MPSQuantizedDecodeRunner (QuantizedDecodeGraphState,
  * mps_kernels.mm:2982-3738, bound at :4373-4461).  The runner keeps pointers to
