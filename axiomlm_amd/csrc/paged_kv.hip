@@ -7,8 +7,8 @@ int paged_view(const axm_paged_kv* d, const char* who, PagedKv* out) {
   AXM_CHECK_ARG(d->kv_dtype >= 0 && d->kv_dtype <= 2, -1, "%s: bad kv dtype %d", who, d->kv_dtype);
   const bool quant = d->kv_dtype != AXM_KV_FP16;
   AXM_CHECK_ARG(!quant || (d->k_scales && d->v_scales), -1, "%s: quantized cache needs scales", who);
-  AXM_CHECK_ARG(d->page_size >= 8 && d->page_size <= 1024 && (d->page_size & (d->page_size - 1)) == 0, -1,
-                "%s: page_size=%d must be a power of two between 8 and 1024", who, d->page_size);
+  AXM_CHECK_ARG(d->page_size >= 16 && d->page_size <= 1024 && (d->page_size & (d->page_size - 1)) == 0, -1,
+                "%s: page_size=%d must be a power of two between 16 and 1024", who, d->page_size);
   AXM_CHECK_ARG(d->n_kv_head >= 1 && d->n_kv_head <= 1024 && d->n_pages >= 1 && d->n_seqs >= 1 && d->max_pages >= 1, -1,
                 "%s: bad cache shape (%d KV heads, %d pages, %d sequences of %d pages)", who, d->n_kv_head, d->n_pages,
                 d->n_seqs, d->max_pages);

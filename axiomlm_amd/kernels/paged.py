@@ -8,7 +8,7 @@ indexing).  All compute runs in libaxm.so.
 A layer's pages are ``k_cache`` / ``v_cache`` (P, Hkv, page_size, width): fp16 with width hd, or uint8 codes (FP8
 E4M3FN: hd, INT4: hd/2) with fp16 ``k_scales`` / ``v_scales`` (P, Hkv, page_size, hd/64).  Pages may be strided (a view of a
 larger pool); what is inside a page is contiguous.  ``block_table`` (B, max_pages) int32: slot s of sequence b is row
-``s % page_size`` of page ``block_table[b, s // page_size]``.  Head size 64 or 128, page size a power of two from 8 to
+``s % page_size`` of page ``block_table[b, s // page_size]``.  Head size 64 or 128, page size a power of two from 16 to
 1024.  Table, lengths, positions and slots are read on the device: captured graphs replay with new ones.  Numbers that
 are out of range there (a page outside the pool, a sequence outside the table) are skipped and never followed.
 """

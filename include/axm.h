@@ -266,7 +266,7 @@ int axm_gqa_tree_verify(const void* q, const void* k_cache, const void* v_cache,
  * tensor indexing and is deprecated).  A pool of n_pages pages holds the rows of all sequences: k and v
  * [n_pages][Hkv][page_size][row], rows as in the contiguous caches above (fp16 / FP8 / INT4 codes with
  * scales [n_pages][Hkv][page_size][hd/64]).  Slot s of sequence b is row s % page_size of page
- * block_table[b][s / page_size].  Head size 64 or 128; page_size a power of two, 8 to 1024.  k, v and scale
+ * block_table[b][s / page_size].  Head size 64 or 128; page_size a power of two, 16 to 1024.  k, v and scale
  * pages are 16-byte aligned (scales: 4-byte) and may be spaced further apart than dense ones.
  * Tables, lengths and positions are read on the device, so captured graphs replay with new ones. */
 typedef struct axm_paged_kv {

@@ -76,7 +76,7 @@ def test_ragged_lengths(dev, kv, H, Hkv, hd):
     check_decode(q, k, v, table, lens, ks, vs, kv, mass, again, got_mass)
 
 
-@pytest.mark.parametrize("page", [8, 16, 32, 64, 128, 256, 1024])
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256, 1024])
 @pytest.mark.parametrize("kv", ["fp16", "int4"])
 def test_page_sizes(dev, kv, page):
     lens = [5, 64, 700, 31]
@@ -314,7 +314,7 @@ def test_decode_refusals(dev):
     for args in bad:
         with pytest.raises((ValueError, RuntimeError)):
             K.gqa_paged_decode(*args[:5], **args[5])
-    k12 = torch.zeros(4, 2, 12, 64, device=dev, dtype=torch.float16)
+    k12 = torch.zeros(4, 2, 24, 64, device=dev, dtype=torch.float16)
     with pytest.raises(RuntimeError, match="power of two"):
         K.gqa_paged_decode(q, k12, k12, table, n)
     k96 = torch.zeros(4, 2, 16, 96, device=dev, dtype=torch.float16)
@@ -529,7 +529,7 @@ def check_evict(cache, scales, table, lens, mass, budget, recent):
 
 
 @pytest.mark.parametrize("kv", ["fp16", "fp8", "int4"])
-@pytest.mark.parametrize("hd,page,budget,recent", [(64, 16, 20, 5), (128, 32, 1, 0), (64, 8, 33, 33), (128, 16, 64, 0),
+@pytest.mark.parametrize("hd,page,budget,recent", [(64, 16, 20, 5), (128, 32, 1, 0), (64, 16, 33, 33), (128, 16, 64, 0),
                                                    (64, 64, 1, 1)])
 def test_evict(dev, kv, hd, page, budget, recent):
     print(f"[evict] {kv} {hd} {page} {budget}/{recent}", flush=True)

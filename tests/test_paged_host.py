@@ -22,7 +22,7 @@ def desc(**change):
 
 BAD_DESC = [dict(k=None), dict(v=None), dict(block_table=None), dict(head_dim=96), dict(head_dim=0), dict(kv_dtype=3),
             dict(kv_dtype=-1), dict(kv_dtype=1, k_scales=None), dict(kv_dtype=2, v_scales=None), dict(page_size=12),
-            dict(page_size=4), dict(page_size=2048), dict(n_kv_head=0), dict(n_pages=0), dict(n_seqs=0),
+            dict(page_size=8), dict(page_size=2048), dict(n_kv_head=0), dict(n_pages=0), dict(n_seqs=0),
             dict(max_pages=0), dict(max_pages=1 << 28), dict(page_stride=4080), dict(page_stride=4097), dict(k=P + 8),
             dict(kv_dtype=1, page_stride=2048, scale_stride=60), dict(kv_dtype=1, k_scales=P + 2)]
 
