@@ -44,10 +44,29 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
-__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor((unsigned long long)v, o, 64);
-  return v;
+// One candidate as an integer: larger is earlier in the order.
+__device__ __forceinline__ uint64_t candidate(float z, int i) { return (uint64_t)order_key(z) << 32 | (uint32_t)~i; }
+__device__ __forceinline__ float candidate_z(uint64_t c) { return key_value((uint32_t)(c >> 32)); }
+__device__ __forceinline__ int candidate_at(uint64_t c) { return (int)~(uint32_t)c; }
+
+// Inclusive sums over the wave's lanes, on DPP moves: shifts inside rows of 16, then the rows' last lanes onward.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_add64(uint64_t x) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xF, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CTRL, ROWS, 0xF, true);
+  return x + ((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ uint64_t wave_prefix64(uint64_t x) {
+  x = dpp_add64<0x111, 0xF>(x);  // row_shr:1
+  x = dpp_add64<0x112, 0xF>(x);
+  x = dpp_add64<0x114, 0xF>(x);
+  x = dpp_add64<0x118, 0xF>(x);
+  x = dpp_add64<0x142, 0xA>(x);  // row_bcast:15 into rows 1 and 3
+  return dpp_add64<0x143, 0xC>(x);  // row_bcast:31 into rows 2 and 3
+}
+__device__ __forceinline__ uint64_t lane63(uint64_t x) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), 63) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, 63);
 }
 
 struct Lds {
@@ -59,48 +78,91 @@ struct Lds {
     } bins;
     uint64_t sums[kSums];
   };
-  float z[kList];
-  int at[kList];
-  float sorted_z[kList];
-  int sorted_at[kList];
-  uint64_t red[kWaves];
-  uint64_t total, before;
-  float fred[kWaves], cut_z;
-  int ired[kWaves], cut_i, n, bin, where;
+  uint64_t list[kList];
+  uint64_t red[2][kWaves];
+  uint64_t total, before, cut;
+  int n, bin, where;
 };
 
-// Sum over the workgroup, the same in every thread.
-__device__ __forceinline__ uint64_t block_sum(uint64_t v, Lds& s) {
-  v = wave_sum64(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s.red[threadIdx.x >> 6] = v;
+// Sum over the workgroup, the same in every thread.  turn: 0 and 1 in turn, so that one barrier is enough.
+__device__ __forceinline__ uint64_t block_sum(uint64_t v, Lds& s, int& turn) {
+  const uint64_t x = wave_prefix64(v);
+  uint64_t* red = s.red[turn ^= 1];
+  if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = x;
   __syncthreads();
   uint64_t t = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) t += s.red[w];
+  for (int w = 0; w < kWaves; ++w) t += red[w];
   return t;
 }
 
 // Sum over the threads before this one; *total over all.
-__device__ __forceinline__ uint64_t block_before(uint64_t v, Lds& s, uint64_t* total) {
+__device__ __forceinline__ uint64_t block_before(uint64_t v, Lds& s, int& turn, uint64_t* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint64_t x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t y = __shfl_up((unsigned long long)x, o, 64);
-    x += lane >= o ? y : 0;
-  }
-  __syncthreads();
-  if (lane == 63) s.red[wave] = x;
+  const uint64_t x = wave_prefix64(v);
+  uint64_t* red = s.red[turn ^= 1];
+  if (lane == 63) red[wave] = x;
   __syncthreads();
   uint64_t b = 0, t = 0;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    b += w < wave ? s.red[w] : 0;
-    t += s.red[w];
+    b += w < wave ? red[w] : 0;
+    t += red[w];
   }
   *total = t;
   return b + x - v;
+}
+
+// Largest over the workgroup.
+__device__ __forceinline__ uint64_t block_max(uint64_t v, Lds& s, int& turn) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint64_t y = __shfl_xor((unsigned long long)v, o, 64);
+    v = y > v ? y : v;
+  }
+  uint64_t* red = s.red[turn ^= 1];
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) v = red[w] > v ? red[w] : v;
+  return v;
+}
+
+// s.list[0, n) into descending order (n <= kList); all threads, and a barrier at the end.
+__device__ __forceinline__ void sort_list(Lds& s, int n) {
+  __syncthreads();
+  if (n <= 64) {  // ranks by counting, one wave
+    if (threadIdx.x < 64) {
+      const uint64_t mine = (int)threadIdx.x < n ? s.list[threadIdx.x] : 0;
+      int rank = 0;
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) {
+        const uint64_t c = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(mine >> 32), j) << 32 |
+                           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)mine, j);
+        rank += c > mine;
+      }
+      if ((int)threadIdx.x < n) s.list[rank] = mine;
+    }
+    __syncthreads();
+    return;
+  }
+  int size = 128;
+  while (size < n) size *= 2;
+  for (int i = n + threadIdx.x; i < size; i += kThreads) s.list[i] = 0;  // less than every candidate
+  __syncthreads();
+  for (int k = 2; k <= size; k *= 2)  // bitonic
+    for (int j = k / 2; j > 0; j /= 2) {
+      const int t = threadIdx.x;
+      if (t < size / 2) {
+        const int a = (t & ~(j - 1)) * 2 + (t & (j - 1)), b = a + j;
+        const uint64_t x = s.list[a], y = s.list[b];
+        if ((x < y) == ((a & k) == 0)) {
+          s.list[a] = y;
+          s.list[b] = x;
+        }
+      }
+      __syncthreads();
+    }
 }
 
 template <int DT>
@@ -109,6 +171,7 @@ struct Row {
   const u32x4* base;                         // the row's first logit is number `lead` from here
   int lead, V, vectors, tile0, tile1;        // tiles (64 loads) of this wave: a contiguous run
   bool inf;                                  // +inf among them: those count 0, all others -inf
+  u32x4 first[4];                            // the wave's first four tiles stay in registers
 
   // Loads stay inside the 16-byte blocks that hold the row's first and last logits.
   __device__ __forceinline__ u32x4 load(int tile) const {
@@ -143,16 +206,15 @@ struct Row {
   // f(tile, z) for every tile of this wave, four loads on their way.
   template <typename F>
   __device__ __forceinline__ void pass(const F& f) const {
+    u32x4 r[4] = {first[0], first[1], first[2], first[3]};
 #pragma unroll 1
     for (int t = tile0; t < tile1; t += 4) {
-      u32x4 r[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) r[k] = load(min(t + k, tile1 - 1));
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if (t + k < tile1) {
           float z[E];
           values(t + k, r[k], z);
+          if (t + k + 4 < tile1) r[k] = load(t + k + 4);
           f(t + k, z);
         }
       }
@@ -180,11 +242,12 @@ struct Weight {
   }
 };
 
-// The first logit, in index order, at which the running sum of f passes `target` (by the order of sums as doubles where
-// target is no integer), or the last one with a weight.  -> its index in s.where, its f in s.before; s.total the sum.
-// f(z, i) >= 0; frac: target is that share of the total.
+// The first logit, in index order, at which the running sum of weights passes `target` (sums compared as doubles), or the
+// last one with a weight.  -> its index in s.where, its weight in s.before, all weights' sum in s.total.
+// f(tile, z, add) calls add(j, weight) for the tile's logits that have one; frac >= 0: target is that share of the sum.
 template <int DT, typename F>
-__device__ __forceinline__ void find_in_order(const Row<DT>& row, Lds& s, const F& f, double frac, double target) {
+__device__ __forceinline__ void find_in_order(const Row<DT>& row, Lds& s, int& turn, const F& f, double frac,
+                                              double target) {
   constexpr int E = Row<DT>::E;
   const int lane = threadIdx.x & 63;
   const int tiles = (row.vectors + 63) / 64, group = (tiles + kSums - 1) / kSums;
@@ -193,11 +256,10 @@ __device__ __forceinline__ void find_in_order(const Row<DT>& row, Lds& s, const 
   __syncthreads();
   row.pass([&](int tile, const float (&z)[E]) {
     uint64_t w = 0;
-#pragma unroll
-    for (int j = 0; j < E; ++j) w += f(z[j], row.index(tile, j));
+    f(tile, z, [&](int, uint64_t x) { w += x; });
     if (__builtin_amdgcn_ballot_w64(w != 0)) {
-      w = wave_sum64(w);
-      if (lane == 0) atomicAdd((unsigned long long*)&s.sums[tile / group], (unsigned long long)w);
+      w = wave_prefix64(w);
+      if (lane == 63) atomicAdd((unsigned long long*)&s.sums[tile / group], (unsigned long long)w);
     }
   });
   __syncthreads();
@@ -205,13 +267,15 @@ __device__ __forceinline__ void find_in_order(const Row<DT>& row, Lds& s, const 
   uint64_t e[kEach], mine = 0, total;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) mine += e[i] = s.sums[threadIdx.x * kEach + i];
-  uint64_t run = block_before(mine, s, &total);
+  uint64_t run = block_before(mine, s, turn, &total);
   if (frac >= 0.0) target = frac * (double)total;
   // Sums as doubles never fall, so one entry passes the target; or none does, and the last with a weight counts.
-  auto passes = [&](uint64_t sum) { return (double)sum > target || sum == total; };
+  auto passes = [&](uint64_t before, uint64_t w) {
+    return w != 0 && ((double)(before + w) > target || before + w == total) && !((double)before > target);
+  };
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
-    if (e[i] != 0 && passes(run + e[i]) && !((double)run > target) && run != total) {
+    if (passes(run, e[i])) {
       s.n = threadIdx.x * kEach + i;
       s.before = run;
     }
@@ -227,19 +291,15 @@ __device__ __forceinline__ void find_in_order(const Row<DT>& row, Lds& s, const 
       row.values(tile, row.load(tile), z);
       uint64_t w[E], sum = 0;
 #pragma unroll
-      for (int j = 0; j < E; ++j) sum += w[j] = f(z[j], row.index(tile, j));
-      uint64_t x = sum;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t y = __shfl_up((unsigned long long)x, o, 64);
-        x += lane >= o ? y : 0;
-      }
-      const uint64_t after = run + __shfl((unsigned long long)x, 63, 64);
+      for (int j = 0; j < E; ++j) w[j] = 0;
+      f(tile, z, [&](int j, uint64_t x) { sum += w[j] = x; });
+      const uint64_t x = wave_prefix64(sum);
       uint64_t here = run + x - sum;
+      run += lane63(x);
       bool hit = false;
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        if (w[j] != 0 && passes(here + w[j]) && !((double)here > target) && here != total) {
+        if (passes(here, w[j])) {
           hit = true;
           s.where = row.index(tile, j);
           s.total = total;
@@ -248,7 +308,6 @@ __device__ __forceinline__ void find_in_order(const Row<DT>& row, Lds& s, const 
         here += w[j];
       }
       found = __builtin_amdgcn_ballot_w64(hit) != 0;
-      run = after;
     }
   }
   __syncthreads();
@@ -275,45 +334,39 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
   const float min_p = p.min_p ? p.min_p[r] : p.min_p_all;
   const double u = fmin(fmax((double)p.u[r], 0.0), 1.0);  // (NaN: 0)
 
+  int turn = 0;
   auto answer = [&](int token, float prob) {
     p.tokens[r] = token;
     if (p.probs) p.probs[r] = prob;
   };
+  if (row.tile0 < row.tile1) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) row.first[k] = row.load(min(row.tile0 + k, row.tile1 - 1));
+  }
+  const bool greedy = !(temperature > 0.f);
+  const int k = top_k > 0 && top_k < p.V ? top_k : 0;
+  if (!greedy) {
+    if (threadIdx.x < 256) s.table[threadIdx.x] = exp2((double)p.shift - threadIdx.x * (1.0 / 256));
+    if (k > 0)
+      for (int i = threadIdx.x; i < kBins; i += kThreads) s.bins.count[i] = 0;
+    if (threadIdx.x == 0) s.n = 0, s.bin = -1;
+  }
 
   // ---- the largest logit, lowest index ----
   float top = -INFINITY;
   int top_at = -1;
   row.pass([&](int tile, const float (&z)[E]) {
 #pragma unroll
-    for (int j = 0; j < E; ++j)
-      if (z[j] > top) {
-        top = z[j];
-        top_at = row.index(tile, j);
-      }
+    for (int j = 0; j < E; ++j) {
+      const bool more = z[j] > top;
+      top = more ? z[j] : top;
+      top_at = more ? row.index(tile, j) : top_at;
+    }
   });
-  auto better = [](float z, int i, float z2, int i2) { return z2 > z || (z2 == z && (unsigned)i2 < (unsigned)i); };
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float z2 = __shfl_xor(top, o, 64);
-    const int i2 = __shfl_xor(top_at, o, 64);
-    if (better(top, top_at, z2, i2)) {
-      top = z2;
-      top_at = i2;
-    }
-  }
-  if (lane == 0) {
-    s.fred[wave] = top;
-    s.ired[wave] = top_at;
-  }
-  if (threadIdx.x < 256) s.table[threadIdx.x] = exp2((double)p.shift - threadIdx.x * (1.0 / 256));
-  __syncthreads();
-  for (int w = 0; w < kWaves; ++w)
-    if (better(top, top_at, s.fred[w], s.ired[w])) {
-      top = s.fred[w];
-      top_at = s.ired[w];
-    }
-  if (top_at < 0 || !(temperature > 0.f)) {  // nothing to take; greedy
-    if (threadIdx.x == 0) answer(top_at, top_at < 0 ? 0.f : 1.f);
+  const uint64_t best = block_max(top_at < 0 ? 0 : candidate(top, top_at), s, turn);
+  top = candidate_z(best);
+  if (best == 0 || greedy) {  // nothing to take; the largest
+    if (threadIdx.x == 0) answer(best == 0 ? -1 : candidate_at(best), best == 0 ? 0.f : 1.f);
     return;
   }
   if (top == INFINITY) {
@@ -324,45 +377,37 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
   const uint64_t largest = 1ull << p.shift;
   const double least = (double)min_p * (double)largest;
   auto stays = [&](uint64_t w) { return (double)w >= least || w == largest; };  // min-p
-  float cut_z = -INFINITY;  // kept: z > cut_z, or z == cut_z and i <= cut_i
+  // Kept: z > cut_z, or z == cut_z and i <= cut_i; without a cut, what is over -inf.
+  float cut_z = -INFINITY;
   int cut_i = -1;
-  auto kept = [&](float z, int i) { return z > cut_z || (z == cut_z && i <= cut_i); };
+  auto kept = [&](float z, int tile, int j) {
+    return z > cut_z || (z == cut_z && row.index(tile, j) <= cut_i);
+  };
 
   // The cut inside bin `bin`, whose kept logits are too many for the list: by value first, then by index among equal ones.
   // measure(z): what a logit adds; everything before the bin adds `before`; the cut is the logit that reaches `need`.
   auto bisect = [&](int bin, uint64_t before, double need, auto measure) {
-    uint32_t lo = ~0u, hi = 0;
+    uint64_t ends = 0;  // largest of the order and of its complement
+    uint32_t lo = 0, hi = 0;
     row.pass([&](int tile, const float (&z)[E]) {
 #pragma unroll
       for (int j = 0; j < E; ++j)
-        if (kept(z[j], row.index(tile, j)) && bin_of(top, z[j]) == bin) {
-          lo = min(lo, order_key(z[j]));
+        if (kept(z[j], tile, j) && bin_of(top, z[j]) == bin) {
+          lo = max(lo, ~order_key(z[j]));
           hi = max(hi, order_key(z[j]));
         }
     });
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      lo = min(lo, (uint32_t)__shfl_xor((int)lo, o, 64));
-      hi = max(hi, (uint32_t)__shfl_xor((int)hi, o, 64));
-    }
-    __syncthreads();
-    if (lane == 0) {
-      s.ired[wave] = (int)lo;
-      s.fred[wave] = __builtin_bit_cast(float, hi);
-    }
-    __syncthreads();
-    for (int w = 0; w < kWaves; ++w) {
-      lo = min(lo, (uint32_t)s.ired[w]);
-      hi = max(hi, __builtin_bit_cast(uint32_t, s.fred[w]));
-    }
+    ends = block_max(lo, s, turn);
+    lo = ~(uint32_t)ends;
+    hi = (uint32_t)block_max(hi, s, turn);
     auto from = [&](uint32_t key) {  // measured in the bin at or over key
       uint64_t a = 0;
       row.pass([&](int tile, const float (&z)[E]) {
 #pragma unroll
         for (int j = 0; j < E; ++j)
-          if (kept(z[j], row.index(tile, j)) && bin_of(top, z[j]) == bin && order_key(z[j]) >= key) a += measure(z[j]);
+          if (kept(z[j], tile, j) && bin_of(top, z[j]) == bin && order_key(z[j]) >= key) a += measure(z[j]);
       });
-      return before + block_sum(a, s);
+      return before + block_sum(a, s, turn);
     };
     while (lo < hi) {  // the largest key that reaches `need`
       const uint32_t mid = lo + (hi - lo) / 2 + 1;
@@ -372,17 +417,17 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
     const float z_cut = key_value(lo);
     const double over = (double)from(lo + 1), each = (double)measure(z_cut);
     const double rank = fmax(ceil((need - over) / each), 1.0);  // of those equal to it
-    find_in_order<DT>(row, s, [&](float z, int i) { return (uint64_t)(z == z_cut && kept(z, i)); }, -1.0, rank - 1.0);
+    find_in_order<DT>(row, s, turn, [&](int tile, const float (&z)[E], auto add) {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (z[j] == z_cut && kept(z[j], tile, j)) add(j, 1);
+    }, -1.0, rank - 1.0);
     cut_z = z_cut;
     cut_i = s.where;
   };
 
   // ---- top-k ----
-  const int k = top_k > 0 && top_k < p.V ? top_k : 0;
   if (k > 0) {
-    for (int i = threadIdx.x; i < kBins; i += kThreads) s.bins.count[i] = 0;
-    if (threadIdx.x == 0) s.n = 0, s.bin = -1;
-    __syncthreads();
     row.pass([&](int tile, const float (&z)[E]) {
 #pragma unroll
       for (int j = 0; j < E; ++j)
@@ -391,7 +436,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
     __syncthreads();
     uint64_t all;
     const uint32_t c0 = s.bins.count[2 * threadIdx.x], c1 = s.bins.count[2 * threadIdx.x + 1];
-    const uint64_t before = block_before(c0 + c1, s, &all);
+    const uint64_t before = block_before(c0 + c1, s, turn, &all);
     if (before < (uint64_t)k && before + c0 + c1 >= (uint64_t)k) {
       const bool second = before + c0 < (uint64_t)k;
       s.bin = 2 * threadIdx.x + second;
@@ -402,70 +447,76 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
       const int bin = s.bin >= 0 ? s.bin : kBins - 1;
       const uint64_t ahead = s.bin >= 0 ? s.before : all, upto = s.bin >= 0 ? ahead + s.bins.count[bin] : all;
       const bool whole = upto <= (uint64_t)kList;  // the list takes all candidates, not just the bin with the cut
-      const int least_bin = whole ? 0 : bin;
-      const uint64_t listed = whole ? upto : upto - ahead;
-      if (listed <= (uint64_t)kList) {
+      if (whole || upto - ahead <= (uint64_t)kList) {
+        const int least_bin = whole ? 0 : bin;
         row.pass([&](int tile, const float (&z)[E]) {
 #pragma unroll
           for (int j = 0; j < E; ++j) {
             const int b = bin_of(top, z[j]);
-            if (z[j] > -INFINITY && b >= least_bin && b <= bin) {
-              const int at = atomicAdd(&s.n, 1);
-              s.z[at] = z[j];
-              s.at[at] = row.index(tile, j);
-            }
+            if (b <= bin && b >= least_bin && z[j] > -INFINITY)
+              s.list[atomicAdd(&s.n, 1)] = candidate(z[j], row.index(tile, j));
           }
         });
         __syncthreads();
         const int n = s.n;
-        for (int i = threadIdx.x; i < n; i += kThreads) {
-          const float z = s.z[i];
-          const int at = s.at[i];
-          int rank = 0;
-          for (int j = 0; j < n; ++j) rank += s.z[j] > z || (s.z[j] == z && s.at[j] < at);
-          s.sorted_z[rank] = z;
-          s.sorted_at[rank] = at;
-        }
-        __syncthreads();
+        sort_list(s, n);
         if (!whole) {
-          cut_z = s.sorted_z[k - 1 - (int)ahead];
-          cut_i = s.sorted_at[k - 1 - (int)ahead];
+          const uint64_t c = s.list[k - 1 - (int)ahead];
+          cut_z = candidate_z(c);
+          cut_i = candidate_at(c);
         } else {
-          // All that is left happens on the list: ranks below `last` stay.
+          // All that is left happens on the list, two neighbouring ranks a thread.
           const int m = min(n, k);
-          uint64_t w[2] = {0, 0}, sum;
+          uint64_t c[2] = {0, 0}, w[2] = {0, 0}, sum;
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            if (2 * (int)threadIdx.x + e < m) w[e] = weight(s.sorted_z[2 * threadIdx.x + e]);
-          const uint64_t ahead_w = block_before(w[0] + w[1], s, &sum);
+            if (2 * (int)threadIdx.x + e < m) {
+              c[e] = s.list[2 * threadIdx.x + e];
+              w[e] = weight(candidate_z(c[e]));
+            }
+          const uint64_t ahead_w = block_before(w[0] + w[1], s, turn, &sum);
           const double need = top_p < 1.f ? (double)top_p * (double)sum : INFINITY;
-          uint64_t mine = 0;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int i = 2 * threadIdx.x + e;
-            const uint64_t b = ahead_w + (e ? w[0] : 0);
-            const bool in = i < m && (i == 0 || (double)b < need) && stays(w[e]);
-            mine += in ? 1 : 0;
-          }
-          const int last = (int)block_sum(mine, s);  // weights fall with the rank, so the kept ranks are the first ones
-          uint64_t kept_w = 0;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) kept_w += 2 * (int)threadIdx.x + e < last ? w[e] : 0;
-          const uint64_t total = block_sum(kept_w, s);
-          uint64_t* ws = s.sums;
+          // Sums rise and weights fall with the rank, so the kept ranks are the first ones; the others weigh 0.
+          const int i0 = 2 * (int)threadIdx.x;
+          const bool in0 = i0 < m && (i0 == 0 || (double)ahead_w < need) && stays(w[0]);
+          const bool in1 = i0 + 1 < m && (double)(ahead_w + w[0]) < need && stays(w[1]);
+          w[0] = in0 ? w[0] : 0;
+          w[1] = in1 ? w[1] : 0;
+          const uint64_t total = block_sum(w[0] + w[1], s, turn);
+          const double target = u * (double)total;
+          // Running sums in index order, by 1024 stretches of the vocabulary, then inside the one that passes the target.
+          const int each = (p.V + kThreads - 1) / kThreads;
+          s.sums[threadIdx.x] = 0;
+          if (threadIdx.x == 0) s.n = 0;
+          __syncthreads();
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            if (2 * (int)threadIdx.x + e < last) ws[2 * threadIdx.x + e] = w[e];
+            if (w[e] != 0) atomicAdd((unsigned long long*)&s.sums[candidate_at(c[e]) / each], (unsigned long long)w[e]);
           __syncthreads();
-          const double target = u * (double)total;
-          for (int i = threadIdx.x; i < last; i += kThreads) {
-            const uint64_t mine_w = ws[i];
-            const int at = s.sorted_at[i];
-            uint64_t upto_w = 0;
-            for (int j = 0; j < last; ++j) upto_w += s.sorted_at[j] <= at ? ws[j] : 0;
-            const bool hit = (double)upto_w > target || upto_w == total;
-            if (mine_w != 0 && hit && !((double)(upto_w - mine_w) > target) && upto_w - mine_w != total)
-              answer(at, (float)((double)mine_w / (double)total));
+          uint64_t total2;
+          const uint64_t mine = s.sums[threadIdx.x], run = block_before(mine, s, turn, &total2);
+          auto passes = [&](uint64_t b, uint64_t x) {
+            return x != 0 && ((double)(b + x) > target || b + x == total) && !((double)b > target);
+          };
+          if (passes(run, mine)) {
+            s.where = threadIdx.x;
+            s.before = run;
+          }
+          __syncthreads();
+          // (index, weight) of the stretch's candidates; the list itself is in registers.
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (w[e] != 0 && candidate_at(c[e]) / each == s.where) {
+              const int at = atomicAdd(&s.n, 1);
+              s.list[at] = (uint64_t)candidate_at(c[e]);
+              s.sums[at] = w[e];
+            }
+          __syncthreads();
+          const int inside = s.n;
+          for (int i = threadIdx.x; i < inside; i += kThreads) {
+            uint64_t b = s.before;
+            for (int j = 0; j < inside; ++j) b += s.list[j] < s.list[i] ? s.sums[j] : 0;
+            if (passes(b, s.sums[i])) answer((int)s.list[i], (float)((double)s.sums[i] / (double)total));
           }
           return;
         }
@@ -484,13 +535,13 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
     row.pass([&](int tile, const float (&z)[E]) {
 #pragma unroll
       for (int j = 0; j < E; ++j)
-        if (kept(z[j], row.index(tile, j)))
+        if (kept(z[j], tile, j))
           atomicAdd((unsigned long long*)&s.bins.weight[bin_of(top, z[j])], (unsigned long long)weight(z[j]));
     });
     __syncthreads();
     uint64_t all;
     const uint64_t c0 = s.bins.weight[2 * threadIdx.x], c1 = s.bins.weight[2 * threadIdx.x + 1];
-    const uint64_t before = block_before(c0 + c1, s, &all);
+    const uint64_t before = block_before(c0 + c1, s, turn, &all);
     const double need = (double)top_p * (double)all;
     // The first bin whose sum reaches `need` (bin 0 where need is 0).
     if ((double)before < need && (double)(before + c0 + c1) >= need) {
@@ -504,49 +555,45 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
     row.pass([&](int tile, const float (&z)[E]) {
 #pragma unroll
       for (int j = 0; j < E; ++j)
-        if (kept(z[j], row.index(tile, j)) && bin_of(top, z[j]) == bin) {
+        if (bin_of(top, z[j]) == bin && kept(z[j], tile, j)) {
           const int at = atomicAdd(&s.n, 1);
-          if (at < kList) {
-            s.z[at] = z[j];
-            s.at[at] = row.index(tile, j);
-          }
+          if (at < kList) s.list[at] = candidate(z[j], row.index(tile, j));
         }
     });
     __syncthreads();
     const int n = s.n;
     if (n <= kList) {
-      for (int i = threadIdx.x; i < n; i += kThreads) {
-        const float z = s.z[i];
-        const int at = s.at[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += s.z[j] > z || (s.z[j] == z && s.at[j] < at);
-        s.sorted_z[rank] = z;
-        s.sorted_at[rank] = at;
-      }
-      __syncthreads();
+      sort_list(s, n);
       uint64_t w[2] = {0, 0}, sum, mine = 0;
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        if (2 * (int)threadIdx.x + e < n) w[e] = weight(s.sorted_z[2 * threadIdx.x + e]);
-      const uint64_t b = ahead + block_before(w[0] + w[1], s, &sum);
+        if (2 * (int)threadIdx.x + e < n) w[e] = weight(candidate_z(s.list[2 * threadIdx.x + e]));
+      const uint64_t b = ahead + block_before(w[0] + w[1], s, turn, &sum);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int i = 2 * threadIdx.x + e;
         mine += i < n && (i == 0 || (double)(b + (e ? w[0] : 0)) < need) ? 1 : 0;
       }
-      const int last = (int)block_sum(mine, s) - 1;  // sums never fall, so the kept ranks are the first ones
-      cut_z = s.sorted_z[last];
-      cut_i = s.sorted_at[last];
+      const uint64_t c = s.list[(int)block_sum(mine, s, turn) - 1];  // sums never fall: the kept ranks are the first ones
+      cut_z = candidate_z(c);
+      cut_i = candidate_at(c);
     } else {
       bisect(bin, ahead, need, weight);
     }
   }
 
   // ---- the token ----
-  find_in_order<DT>(row, s, [&](float z, int i) -> uint64_t {
-    if (!kept(z, i)) return 0;
-    const uint64_t w = weight(z);
-    return stays(w) ? w : 0;
+  find_in_order<DT>(row, s, turn, [&](int tile, const float (&z)[E], auto add) {
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < E; ++j) any |= z[j] >= cut_z;
+    if (!__builtin_amdgcn_ballot_w64(any)) return;
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if (kept(z[j], tile, j)) {
+        const uint64_t w = weight(z[j]);
+        if (stays(w)) add(j, w);
+      }
   }, u, 0.0);
   if (threadIdx.x == 0) answer(s.where, (float)((double)s.before / (double)s.total));
 }
