@@ -18,7 +18,31 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 2048;
 constexpr float kBinsPerUnit = 64.f;
 constexpr int kList = 2048;  // candidates in LDS
+#ifndef AH
+#define AH 2
+#endif
+constexpr int kAhead = AH;
 constexpr int kSums = 3072;  // entries of the running sum
+
+// 2^(j / 64), rounded to nearest.
+__device__ const double kOctave[64] = {
+    1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
+    1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
+    1.0905077326652577, 1.1023825833078409, 1.1143867425958924, 1.1265216186082418,
+    1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812,
+    1.189207115002721, 1.2021567314527031, 1.215247359980469, 1.22848053610687,
+    1.241857812073484, 1.2553807570246911, 1.2690509571917332, 1.2828700160787783,
+    1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.3396675240533029,
+    1.3542555469368927, 1.3690024229745905, 1.383909881963832, 1.3989796725383112,
+    1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647,
+    1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384,
+    1.5422108254079407, 1.5590044002378369, 1.5759808451078865, 1.593142151342267,
+    1.6104903319492543, 1.6280274218573478, 1.6457554781539649, 1.6636765803267364,
+    1.681792830507429, 1.7001063537185235, 1.7186192981224779, 1.7373338352737062,
+    1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
+    1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
+    1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.9784560263879509,
+};
 
 struct SampleParams {
   const void* logits;
@@ -70,7 +94,7 @@ __device__ __forceinline__ uint64_t lane63(uint64_t x) {
 }
 
 struct Lds {
-  double table[256];  // 2^(shift - j / 256)
+  double table[64];  // of 2^(j / 64)
   union {
     struct {
       uint64_t weight[kBins];
@@ -114,33 +138,47 @@ __device__ __forceinline__ uint64_t block_before(uint64_t v, Lds& s, int& turn, 
 }
 
 // Largest over the workgroup.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_max64(uint64_t x) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xF, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CTRL, ROWS, 0xF, true);
+  const uint64_t y = (uint64_t)hi << 32 | lo;
+  return y > x ? y : x;
+}
 __device__ __forceinline__ uint64_t block_max(uint64_t v, Lds& s, int& turn) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint64_t y = __shfl_xor((unsigned long long)v, o, 64);
-    v = y > v ? y : v;
-  }
+  v = dpp_max64<0x111, 0xF>(v);
+  v = dpp_max64<0x112, 0xF>(v);
+  v = dpp_max64<0x114, 0xF>(v);
+  v = dpp_max64<0x118, 0xF>(v);
+  v = dpp_max64<0x142, 0xA>(v);
+  v = dpp_max64<0x143, 0xC>(v);
   uint64_t* red = s.red[turn ^= 1];
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = v;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) v = red[w] > v ? red[w] : v;
   return v;
 }
 
+__device__ __forceinline__ uint64_t of_lane(uint64_t x, int j) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), j) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, j);
+}
+// Place of a lane's candidate among the n <= 64 of the wave's first lanes.
+__device__ __forceinline__ int rank_in_wave(uint64_t mine, int n) {
+  int rank = 0;
+#pragma unroll 4
+  for (int j = 0; j < n; ++j) rank += of_lane(mine, j) > mine;
+  return rank;
+}
+
 // s.list[0, n) into descending order (n <= kList); all threads, and a barrier at the end.
 __device__ __forceinline__ void sort_list(Lds& s, int n) {
   __syncthreads();
-  if (n <= 64) {  // ranks by counting, one wave
+  if (n <= 64) {
     if (threadIdx.x < 64) {
       const uint64_t mine = (int)threadIdx.x < n ? s.list[threadIdx.x] : 0;
-      int rank = 0;
-#pragma unroll 8
-      for (int j = 0; j < n; ++j) {
-        const uint64_t c = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(mine >> 32), j) << 32 |
-                           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)mine, j);
-        rank += c > mine;
-      }
+      const int rank = rank_in_wave(mine, n);
       if ((int)threadIdx.x < n) s.list[rank] = mine;
     }
     __syncthreads();
@@ -171,7 +209,7 @@ struct Row {
   const u32x4* base;                         // the row's first logit is number `lead` from here
   int lead, V, vectors, tile0, tile1;        // tiles (64 loads) of this wave: a contiguous run
   bool inf;                                  // +inf among them: those count 0, all others -inf
-  u32x4 first[4];                            // the wave's first four tiles stay in registers
+  u32x4 first[kAhead];                       // the wave's first tiles stay in registers
 
   // Loads stay inside the 16-byte blocks that hold the row's first and last logits.
   __device__ __forceinline__ u32x4 load(int tile) const {
@@ -203,18 +241,20 @@ struct Row {
       for (int j = 0; j < E; ++j) z[j] = z[j] == INFINITY ? 0.f : -INFINITY;
     }
   }
-  // f(tile, z) for every tile of this wave, four loads on their way.
+  // f(tile, z) for every tile of this wave, the next kAhead on their way.
   template <typename F>
   __device__ __forceinline__ void pass(const F& f) const {
-    u32x4 r[4] = {first[0], first[1], first[2], first[3]};
-#pragma unroll 1
-    for (int t = tile0; t < tile1; t += 4) {
+    u32x4 r[kAhead];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < kAhead; ++k) r[k] = first[k];
+#pragma unroll 1
+    for (int t = tile0; t < tile1; t += kAhead) {
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
         if (t + k < tile1) {
           float z[E];
           values(t + k, r[k], z);
-          if (t + k + 4 < tile1) r[k] = load(t + k + 4);
+          if (t + k + kAhead < tile1) r[k] = load(t + k + kAhead);
           f(t + k, z);
         }
       }
@@ -226,18 +266,21 @@ __device__ __forceinline__ int bin_of(float top, float z) {  // -inf and NaN: th
   return (int)fminf((top - z) * kBinsPerUnit, (float)(kBins - 1));
 }
 
-// 2^shift 2^(-(top - z) rate) as an integer: the table's 2^(shift - j / 256), times a polynomial of the rest (under
-// 2^-8 octaves: four terms reach 2^-49), rounded by adding 2^52.
+// 2^shift 2^((z - top) rate / 64) as an integer: the table's 2^(j / 64) times a polynomial of the rest, at most
+// 2^-7 octaves either way (four terms: 2^-44 of the weight), rounded by adding 2^52.  z - top and what follows in 64
+// bits: differences of fp32 logits do not fit 32.
 struct Weight {
-  double top, rate;  // rate: 256 log2(e) / T
+  double top, rate;  // rate: 64 log2(e) / T
+  int shift;
   const double* table;
   __device__ __forceinline__ uint64_t operator()(float z) const {
-    const double y = fmin((top - (double)z) * rate, 256.0 * 64.0);
-    const int i = (int)y;
-    const double r = y - (double)i;
-    constexpr double a = 0.0027076061740622863;  // ln 2 / 256
-    const double q = fma(fma(fma(fma(r, a * a * a * a / 24, -a * a * a / 6), r, a * a / 2), r, -a), r, 1.0);
-    const double w = ldexp(table[i & 255] * q, -(i >> 8));
+    const double y = fmax(((double)z - top) * rate, -64.0 * 1024.0);
+    const double near = y + 6755399441055744.0;  // 1.5 2^52: the nearest integer in the low bits
+    const int i = (int)(uint32_t)__builtin_bit_cast(uint64_t, near);
+    const double r = y - (near - 6755399441055744.0);
+    constexpr double a = 0.010830424696249145;  // ln 2 / 64
+    const double q = fma(fma(fma(fma(r, a * a * a * a / 24, a * a * a / 6), r, a * a / 2), r, a), r, 1.0);
+    const double w = ldexp(table[i & 63] * q, (i >> 6) + shift);
     return __builtin_bit_cast(uint64_t, w + 4503599627370496.0) - 0x4330000000000000ull;
   }
 };
@@ -341,12 +384,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
   };
   if (row.tile0 < row.tile1) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) row.first[k] = row.load(min(row.tile0 + k, row.tile1 - 1));
+    for (int k = 0; k < kAhead; ++k) row.first[k] = row.load(min(row.tile0 + k, row.tile1 - 1));
   }
   const bool greedy = !(temperature > 0.f);
   const int k = top_k > 0 && top_k < p.V ? top_k : 0;
   if (!greedy) {
-    if (threadIdx.x < 256) s.table[threadIdx.x] = exp2((double)p.shift - threadIdx.x * (1.0 / 256));
+    if (threadIdx.x < 64) s.table[threadIdx.x] = kOctave[threadIdx.x];
     if (k > 0)
       for (int i = threadIdx.x; i < kBins; i += kThreads) s.bins.count[i] = 0;
     if (threadIdx.x == 0) s.n = 0, s.bin = -1;
@@ -364,6 +407,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
     }
   });
   const uint64_t best = block_max(top_at < 0 ? 0 : candidate(top, top_at), s, turn);
+  const float own = top;
   top = candidate_z(best);
   if (best == 0 || greedy) {  // nothing to take; the largest
     if (threadIdx.x == 0) answer(best == 0 ? -1 : candidate_at(best), best == 0 ? 0.f : 1.f);
@@ -373,15 +417,16 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
     row.inf = true;
     top = 0.f;
   }
-  const Weight weight{(double)top, 256.0 * 1.4426950408889634 / (double)temperature, s.table};
+  const Weight weight{(double)top, 64.0 * 1.4426950408889634 / (double)temperature, p.shift, s.table};
   const uint64_t largest = 1ull << p.shift;
-  const double least = (double)min_p * (double)largest;
-  auto stays = [&](uint64_t w) { return (double)w >= least || w == largest; };  // min-p
+  // min-p: weights from `least` on stay (the largest always).
+  const uint64_t least = (uint64_t)fmin(fmax(ceil((double)min_p * (double)largest), 0.0), (double)largest);
+  auto stays = [&](uint64_t w) { return w >= least; };
   // Kept: z > cut_z, or z == cut_z and i <= cut_i; without a cut, what is over -inf.
   float cut_z = -INFINITY;
   int cut_i = -1;
   auto kept = [&](float z, int tile, int j) {
-    return z > cut_z || (z == cut_z && row.index(tile, j) <= cut_i);
+    return (z > cut_z) | ((z == cut_z) & (j <= cut_i - row.index(tile, 0)));
   };
 
   // The cut inside bin `bin`, whose kept logits are too many for the list: by value first, then by index among equal ones.
@@ -428,37 +473,97 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
 
   // ---- top-k ----
   if (k > 0) {
-    row.pass([&](int tile, const float (&z)[E]) {
-#pragma unroll
-      for (int j = 0; j < E; ++j)
-        if (z[j] > -INFINITY) atomicAdd(&s.bins.count[bin_of(top, z[j])], 1u);
-    });
-    __syncthreads();
-    uint64_t all;
-    const uint32_t c0 = s.bins.count[2 * threadIdx.x], c1 = s.bins.count[2 * threadIdx.x + 1];
-    const uint64_t before = block_before(c0 + c1, s, turn, &all);
-    if (before < (uint64_t)k && before + c0 + c1 >= (uint64_t)k) {
-      const bool second = before + c0 < (uint64_t)k;
-      s.bin = 2 * threadIdx.x + second;
-      s.before = before + (second ? c0 : 0);
-    }
-    __syncthreads();
-    if (s.bin >= 0 || all <= kList) {  // (with no more candidates than k, all of them are kept)
-      const int bin = s.bin >= 0 ? s.bin : kBins - 1;
-      const uint64_t ahead = s.bin >= 0 ? s.before : all, upto = s.bin >= 0 ? ahead + s.bins.count[bin] : all;
-      const bool whole = upto <= (uint64_t)kList;  // the list takes all candidates, not just the bin with the cut
-      if (whole || upto - ahead <= (uint64_t)kList) {
-        const int least_bin = whole ? 0 : bin;
+    const float own_top = top_at < 0 ? -INFINITY : row.inf ? (own == INFINITY ? 0.f : -INFINITY) : own;
+    // The k-th largest of the threads' own largest logits bounds the cut from below: where few pass it, they are all
+    // candidates and no histogram of the row is needed.
+    bool listed = false;
+    uint64_t all = 0;
+    if (k <= kThreads / 4) {
+      if (own_top > -INFINITY) atomicAdd(&s.bins.count[bin_of(top, own_top)], 1u);
+      __syncthreads();
+      const uint32_t c0 = s.bins.count[2 * threadIdx.x], c1 = s.bins.count[2 * threadIdx.x + 1];
+      const uint64_t before = block_before(c0 + c1, s, turn, &all);
+      if (before < (uint64_t)k && before + c0 + c1 >= (uint64_t)k) s.bin = 2 * threadIdx.x + (before + c0 < (uint64_t)k);
+      s.bins.count[2 * threadIdx.x] = s.bins.count[2 * threadIdx.x + 1] = 0;
+      __syncthreads();
+      const float reach = s.bin >= 0 && s.bin < kBins - 1 ? (float)(s.bin + 1) : 0.f;  // (the last bin has no end)
+      if (reach > 0.f) {
         row.pass([&](int tile, const float (&z)[E]) {
+          float most = z[0];
 #pragma unroll
-          for (int j = 0; j < E; ++j) {
-            const int b = bin_of(top, z[j]);
-            if (b <= bin && b >= least_bin && z[j] > -INFINITY)
-              s.list[atomicAdd(&s.n, 1)] = candidate(z[j], row.index(tile, j));
+          for (int j = 1; j < E; ++j) most = fmaxf(most, z[j]);
+          if ((top - most) * kBinsPerUnit < reach) {
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+              if ((top - z[j]) * kBinsPerUnit < reach) {
+                const int at = atomicAdd(&s.n, 1);
+                if (at < kList) s.list[at] = candidate(z[j], row.index(tile, j));
+              }
           }
         });
         __syncthreads();
+        listed = s.n <= kList;
+        __syncthreads();
+      }
+      if (!listed && threadIdx.x == 0) s.n = 0, s.bin = -1;
+      __syncthreads();
+    }
+    if (!listed) {
+      row.pass([&](int tile, const float (&z)[E]) {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (z[j] > -INFINITY) atomicAdd(&s.bins.count[bin_of(top, z[j])], 1u);
+      });
+      __syncthreads();
+      const uint32_t c0 = s.bins.count[2 * threadIdx.x], c1 = s.bins.count[2 * threadIdx.x + 1];
+      const uint64_t before = block_before(c0 + c1, s, turn, &all);
+      if (before < (uint64_t)k && before + c0 + c1 >= (uint64_t)k) {
+        const bool second = before + c0 < (uint64_t)k;
+        s.bin = 2 * threadIdx.x + second;
+        s.before = before + (second ? c0 : 0);
+      }
+      __syncthreads();
+    }
+    if (listed || s.bin >= 0 || all <= kList) {  // (with no more candidates than k, all of them are kept)
+      const int bin = s.bin >= 0 ? s.bin : kBins - 1;
+      const uint64_t ahead = s.bin >= 0 ? s.before : all, upto = s.bin >= 0 ? ahead + s.bins.count[bin] : all;
+      const bool whole = listed || upto <= (uint64_t)kList;  // the list takes all candidates, not just the bin with the cut
+      if (whole || upto - ahead <= (uint64_t)kList) {
+        if (!listed) {
+          const int least_bin = whole ? 0 : bin;
+          row.pass([&](int tile, const float (&z)[E]) {
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+              const int b = bin_of(top, z[j]);
+              if (b <= bin && b >= least_bin && z[j] > -INFINITY)
+                s.list[atomicAdd(&s.n, 1)] = candidate(z[j], row.index(tile, j));
+            }
+          });
+          __syncthreads();
+        }
         const int n = s.n;
+        if (whole && n <= 64) {  // one wave does the rest: a rank a lane
+          if (threadIdx.x >= 64) return;
+          uint64_t c = lane < n ? s.list[lane] : 0;
+          const int rank = rank_in_wave(c, n);
+          if (lane < n) s.list[rank] = c;
+          __builtin_amdgcn_wave_barrier();
+          const int m = min(n, k);
+          c = lane < m ? s.list[lane] : 0;
+          uint64_t w = lane < m ? weight(candidate_z(c)) : 0;
+          const uint64_t upto_w = wave_prefix64(w);
+          const double need = top_p < 1.f ? (double)top_p * (double)lane63(upto_w) : INFINITY;
+          if (!((lane == 0 || (double)(upto_w - w) < need) && stays(w))) w = 0;
+          const uint64_t total = lane63(wave_prefix64(w));
+          const double target = u * (double)total;
+          const int at = candidate_at(c);
+          uint64_t b = 0;  // weights at lower indices
+#pragma unroll 4
+          for (int j = 0; j < m; ++j) b += __builtin_amdgcn_readlane(at, j) < at ? of_lane(w, j) : 0;
+          if (w != 0 && ((double)(b + w) > target || b + w == total) && !((double)b > target))
+            answer(at, (float)((double)w / (double)total));
+          return;
+        }
         sort_list(s, n);
         if (!whole) {
           const uint64_t c = s.list[k - 1 - (int)ahead];
@@ -534,9 +639,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
     __syncthreads();
     row.pass([&](int tile, const float (&z)[E]) {
 #pragma unroll
-      for (int j = 0; j < E; ++j)
-        if (kept(z[j], tile, j))
-          atomicAdd((unsigned long long*)&s.bins.weight[bin_of(top, z[j])], (unsigned long long)weight(z[j]));
+      for (int j = 0; j < E; ++j) {
+        const uint64_t w = weight(z[j]);  // (of all: eight chains side by side)
+        if (kept(z[j], tile, j)) atomicAdd((unsigned long long*)&s.bins.weight[bin_of(top, z[j])], (unsigned long long)w);
+      }
     });
     __syncthreads();
     uint64_t all;
@@ -589,11 +695,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
     for (int j = 0; j < E; ++j) any |= z[j] >= cut_z;
     if (!__builtin_amdgcn_ballot_w64(any)) return;
 #pragma unroll
-    for (int j = 0; j < E; ++j)
-      if (kept(z[j], tile, j)) {
-        const uint64_t w = weight(z[j]);
-        if (stays(w)) add(j, w);
-      }
+    for (int j = 0; j < E; ++j) {
+      const uint64_t w = weight(z[j]);
+      add(j, kept(z[j], tile, j) & stays(w) ? w : 0);
+    }
   }, u, 0.0);
   if (threadIdx.x == 0) answer(s.where, (float)((double)s.before / (double)s.total));
 }
