@@ -106,6 +106,7 @@ struct Lds {
   uint64_t red[2][kWaves];
   uint64_t total, before, cut;
   int n, bin, where;
+  int small[64];
 };
 
 // Sum over the workgroup, the same in every thread.  turn: 0 and 1 in turn, so that one barrier is enough.
@@ -160,27 +161,20 @@ __device__ __forceinline__ uint64_t block_max(uint64_t v, Lds& s, int& turn) {
   return v;
 }
 
-__device__ __forceinline__ uint64_t of_lane(uint64_t x, int j) {
-  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), j) << 32 |
-         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, j);
-}
-// Place of a lane's candidate among the n <= 64 of the wave's first lanes.
-__device__ __forceinline__ int rank_in_wave(uint64_t mine, int n) {
-  int rank = 0;
-#pragma unroll 4
-  for (int j = 0; j < n; ++j) rank += of_lane(mine, j) > mine;
-  return rank;
-}
-
 // s.list[0, n) into descending order (n <= kList); all threads, and a barrier at the end.
 __device__ __forceinline__ void sort_list(Lds& s, int n) {
   __syncthreads();
-  if (n <= 64) {
-    if (threadIdx.x < 64) {
-      const uint64_t mine = (int)threadIdx.x < n ? s.list[threadIdx.x] : 0;
-      const int rank = rank_in_wave(mine, n);
-      if ((int)threadIdx.x < n) s.list[rank] = mine;
-    }
+  if (n <= 64) {  // places by counting: lane i's candidate against four others in every wave
+    const int i = threadIdx.x & 63, j0 = (threadIdx.x >> 6) * 4;
+    if (threadIdx.x < 64) s.small[i] = 0;
+    const uint64_t mine = i < n ? s.list[i] : 0;
+    int over = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) over += j0 + j < n && s.list[j0 + j] > mine;
+    __syncthreads();
+    if (over) atomicAdd(&s.small[i], over);
+    __syncthreads();
+    if (threadIdx.x < 64 && i < n) s.list[s.small[i]] = mine;
     __syncthreads();
     return;
   }
@@ -542,28 +536,6 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
           __syncthreads();
         }
         const int n = s.n;
-        if (whole && n <= 64) {  // one wave does the rest: a rank a lane
-          if (threadIdx.x >= 64) return;
-          uint64_t c = lane < n ? s.list[lane] : 0;
-          const int rank = rank_in_wave(c, n);
-          if (lane < n) s.list[rank] = c;
-          __builtin_amdgcn_wave_barrier();
-          const int m = min(n, k);
-          c = lane < m ? s.list[lane] : 0;
-          uint64_t w = lane < m ? weight(candidate_z(c)) : 0;
-          const uint64_t upto_w = wave_prefix64(w);
-          const double need = top_p < 1.f ? (double)top_p * (double)lane63(upto_w) : INFINITY;
-          if (!((lane == 0 || (double)(upto_w - w) < need) && stays(w))) w = 0;
-          const uint64_t total = lane63(wave_prefix64(w));
-          const double target = u * (double)total;
-          const int at = candidate_at(c);
-          uint64_t b = 0;  // weights at lower indices
-#pragma unroll 4
-          for (int j = 0; j < m; ++j) b += __builtin_amdgcn_readlane(at, j) < at ? of_lane(w, j) : 0;
-          if (w != 0 && ((double)(b + w) > target || b + w == total) && !((double)b > target))
-            answer(at, (float)((double)w / (double)total));
-          return;
-        }
         sort_list(s, n);
         if (!whole) {
           const uint64_t c = s.list[k - 1 - (int)ahead];
@@ -589,6 +561,28 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
           w[1] = in1 ? w[1] : 0;
           const uint64_t total = block_sum(w[0] + w[1], s, turn);
           const double target = u * (double)total;
+          if (m <= 64) {  // the same comparisons of places again, of indices: s.sums are the weights before each
+            if (threadIdx.x < 64) s.sums[threadIdx.x] = 0;
+            if (threadIdx.x < 32) {  // (the pairs of ranks as they lie in registers)
+              s.sums[64 + 2 * threadIdx.x] = w[0];
+              s.sums[65 + 2 * threadIdx.x] = w[1];
+            }
+            __syncthreads();
+            const int j0 = wave * 4;
+            const int at = lane < m ? candidate_at(s.list[lane]) : 0;
+            uint64_t part = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              part += j0 + j < m && candidate_at(s.list[j0 + j]) < at ? s.sums[64 + j0 + j] : 0;
+            if (lane < m && part != 0) atomicAdd((unsigned long long*)&s.sums[lane], (unsigned long long)part);
+            __syncthreads();
+            if (wave == 0 && lane < m) {
+              const uint64_t b = s.sums[lane], x = s.sums[64 + lane];
+              if (x != 0 && ((double)(b + x) > target || b + x == total) && !((double)b > target))
+                answer(at, (float)((double)x / (double)total));
+            }
+            return;
+          }
           // Running sums in index order, by 1024 stretches of the vocabulary, then inside the one that passes the target.
           const int each = (p.V + kThreads - 1) / kThreads;
           s.sums[threadIdx.x] = 0;
