@@ -237,6 +237,11 @@ def stream_of(device=None) -> c_void_p:
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def raw_stream(index: int) -> int:
+    """Handle of the current stream of device `index` (stream_of without the Python objects around it)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def require_gpu(t, what: str) -> None:
     if not (isinstance(t, torch.Tensor) and t.device.type == "cuda"):
         raise RuntimeError(f"{what}: expected a tensor on a ROCm (cuda) device, got {getattr(t, 'device', type(t))}")

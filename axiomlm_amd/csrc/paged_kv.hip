@@ -41,7 +41,7 @@ namespace {
 // RoPE + store.  A lane holds 8 elements (four rotation pairs) of a head row of [q | k | v], hd / 8 lanes a row, a wave
 // 64 / (hd / 8) rows of one token.  fp32 products and sums, one rounding to fp16 (rope_out), then for quantized pages
 // one scale per 64 elements (8 lanes): fp16(amax / 448 | 7) and codes of fp16(x / scale).  Bound by the rows' bytes; with
-// 4 bytes a lane and a row a wave it took 57.8 us for 4001 tokens of 48 rows instead of 26.6.
+// 4 bytes a lane and a row a wave it took 57.8 us for 4001 tokens of 48 rows into FP8 pages instead of 22.8 (4.1 TB/s).
 // ---------------------------------------------------------------------------
 constexpr int kWriteWaves = 4;
 
@@ -160,13 +160,15 @@ void launch_write(bool vec, unsigned grid, hipStream_t s, f16* qkv, int64_t ld, 
 
 // ---------------------------------------------------------------------------
 // Eviction.  Select: one workgroup per (layer, sequence, KV head).  The value that the (budget - recent)-th largest account
-// before the recent slots has comes from three histograms of its ordered bits (11, 11 and 10); then every wave counts
-// and writes the kept slots of its own stretch in order.  Move: one workgroup per (layer, k | v, sequence, KV head)
+// before the recent slots has comes from histograms of its ordered bits (11, 11 and 10; 1024 heads of up to 4096 slots:
+// 27 us, mostly the histograms' atomics; 13 bits at first, or counting two bits a step over keys in registers, took
+// longer); then every wave counts and writes the kept slots of its own stretch in order.  Move: one workgroup per (layer, k | v, sequence, KV head)
 // copies the kept rows down in ascending tiles.  A row never moves up, so what a later tile reads lies behind the
 // tile being written: a tile's loads are under way while the one before is stored.
 // ---------------------------------------------------------------------------
 constexpr int kEvictThreads = 256;
 constexpr int kEvictWaves = kEvictThreads / 64;
+constexpr int kBinBits = 11, kBinsEach = (1 << kBinBits) / kEvictThreads;
 
 // Order of accounts: larger is kept first; -0 counts as 0, NaN as less than every number.
 __device__ __forceinline__ uint32_t account_key(float a) {
@@ -180,8 +182,8 @@ __global__ void __launch_bounds__(kEvictThreads)
                         int n_seqs, int Hkv, int budget, int recent, float* __restrict__ mass_out,
                         int* __restrict__ kept, int* __restrict__ lens_out) {
   constexpr int kHeld = 16;  // keys a lane keeps in registers (4096 slots); the rest is read again
-  __shared__ uint32_t bins[2048];
-  __shared__ int wave_sum_s[kEvictWaves], found_bin, found_before;
+  __shared__ __align__(16) uint32_t bins[kBinsEach * kEvictThreads];
+  __shared__ int wave_sum_s[kEvictWaves], found_bin, found_before, found_count;
   __shared__ int wave_over[kEvictWaves], wave_equal[kEvictWaves];
   const int64_t row = blockIdx.x;
   const int b = (int)(row / Hkv % n_seqs);
@@ -229,17 +231,25 @@ __global__ void __launch_bounds__(kEvictThreads)
   int need = want;             // keys still to take among those that share them
 #pragma unroll 1
   for (int level = 0; level < 3; ++level) {
-    const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, width = level == 2 ? 10 : 11, size = 1 << width;
-    for (int i = threadIdx.x; i < size; i += kEvictThreads) bins[i] = 0;
+    const int shift = level == 0 ? 32 - kBinBits : level == 1 ? 32 - 2 * kBinBits : 0;
+    const uint32_t digit = level == 2 ? (1u << (32 - 2 * kBinBits)) - 1 : (1u << kBinBits) - 1;
+    u32x4* all = reinterpret_cast<u32x4*>(bins);
+#pragma unroll
+    for (int i = 0; i < kBinsEach / 4; ++i) all[i * kEvictThreads + threadIdx.x] = u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
     pass([&](int, uint32_t key, bool in) {
-      if (in && (key & mask) == cut) atomicAdd(&bins[(key >> shift) & (size - 1)], 1u);
+      if (in && (key & mask) == cut) atomicAdd(&bins[(key >> shift) & digit], 1u);
     });
     __syncthreads();
-    // From the largest bin down: thread t has the bins size - 1 - t per ... size - per - t per.
-    const int per = size / kEvictThreads;
+    // From the largest bin down: thread t has kBinsEach of them.
+    const int first = kEvictThreads - 1 - threadIdx.x;
+    u32x4 c[kBinsEach / 4];
     int mine = 0;
-    for (int i = 0; i < per; ++i) mine += (int)bins[size - 1 - threadIdx.x * per - i];
+#pragma unroll
+    for (int i = 0; i < kBinsEach / 4; ++i) {
+      c[i] = all[first * (kBinsEach / 4) + i];
+      mine += (int)(c[i].x + c[i].y + c[i].z + c[i].w);
+    }
     int x = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -249,17 +259,30 @@ __global__ void __launch_bounds__(kEvictThreads)
     if (lane == 63) wave_sum_s[wave] = x;
     __syncthreads();
     int before = x - mine;
-    for (int w = 0; w < wave; ++w) before += wave_sum_s[w];
+#pragma unroll
+    for (int w = 0; w < kEvictWaves; ++w) before += w < wave ? wave_sum_s[w] : 0;
     if (before < need && before + mine >= need) {
-      int i = 0;
-      while (before + (int)bins[size - 1 - threadIdx.x * per - i] < need) before += (int)bins[size - 1 - threadIdx.x * per - i++];
-      found_bin = size - 1 - threadIdx.x * per - i;
+      int bin = -1, count = 0;
+#pragma unroll
+      for (int i = kBinsEach - 1; i >= 0; --i)
+        if (bin < 0) {
+          count = (int)c[i / 4][i & 3];
+          if (before + count >= need) bin = kBinsEach * first + i;
+          else before += count;
+        }
+      found_bin = bin;
       found_before = before;
+      found_count = count;
     }
     __syncthreads();
     cut |= (uint32_t)found_bin << shift;
-    mask |= (uint32_t)(size - 1) << shift;
+    mask |= digit << shift;
     need -= found_before;
+    if (found_count == need && cut != 0) {  // all that share these bits stay: everything over the key below them
+      --cut;
+      need = 0;
+      break;
+    }
   }
   // `need` of the keys equal to the cut stay, the lowest slots first.
   int over = 0, equal = 0;

@@ -25,11 +25,12 @@ def _kv_code(kv_dtype: str) -> int:
         raise ValueError(f"unsupported kv_dtype {kv_dtype!r}") from None
 
 
-def on_device(device: torch.device):
-    """Makes the tensors' device the current one, for launches on its stream."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def on_device(index: int):
+    """Makes device `index`, the tensors' own, the current one for launches on its stream."""
+    return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _check_head_dim(head_dim: int, who: str) -> None:
@@ -357,15 +358,19 @@ _LOGIT_CODES = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 2}
 
 def _setting(who: str, name: str, x, dtype: torch.dtype, rows: int, device, low: float, high: float):
     """A sampling setting of every row: (device array or None, value)."""
-    if isinstance(x, torch.Tensor) and x.dim() > 0:
-        if x.device != device or x.numel() != rows:
-            raise ValueError(f"{who}: {name} must have one entry per row ({rows}) on {device}, got {tuple(x.shape)} on "
-                             f"{x.device}")
-        return x.to(dtype).contiguous(), 0
-    x = x.item() if isinstance(x, torch.Tensor) else x
+    if isinstance(x, torch.Tensor):
+        if x.dim() > 0:
+            if x.device != device or x.numel() != rows:
+                raise ValueError(f"{who}: {name} must have one entry per row ({rows}) on {device}, got "
+                                 f"{tuple(x.shape)} on {x.device}")
+            return x.to(dtype).contiguous(), 0
+        x = x.item()
     if not low <= x <= high:
         raise ValueError(f"{who}: {name}={x} outside [{low}, {high}]")
     return None, x
+
+
+_INF = float("inf")
 
 
 def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
@@ -380,31 +385,35 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
     probability exceeds the uniform number.  -inf and NaN logits are never taken; +inf ones are taken alone.  A row with
     nothing to take gives -1.  return_probs: also the token's probability among the kept, fp32."""
     who = "sample_tokens"
-    _lib.require_gpu(logits, who)
-    if logits.dtype not in _LOGIT_CODES or logits.dim() < 1 or logits.size(-1) < 1:
-        raise ValueError(f"{who}: logits must be fp16, fp32 or bf16 (..., V), got {tuple(logits.shape)} {logits.dtype}")
-    V = logits.size(-1)
-    lead = logits.shape[:-1]
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+        _lib.require_gpu(logits, who)
+    code = _LOGIT_CODES.get(logits.dtype)
+    shape = logits.shape
+    if code is None or not shape or shape[-1] < 1:
+        raise ValueError(f"{who}: logits must be fp16, fp32 or bf16 (..., V), got {tuple(shape)} {logits.dtype}")
+    V, lead, dev = shape[-1], shape[:-1], logits.device
     rows = logits.numel() // V
-    dev = logits.device
     if not isinstance(uniforms, torch.Tensor) or uniforms.device != dev or uniforms.dtype != torch.float32 \
             or uniforms.numel() != rows:
         raise ValueError(f"{who}: uniforms must be fp32, one per row ({rows}) on {dev}")
-    inf = float("inf")
-    t, t_all = _setting(who, "temperature", temperature, torch.float32, rows, dev, 0.0, inf)
-    k, k_all = _setting(who, "top_k", top_k, torch.int32, rows, dev, 0, inf)
+    t, t_all = _setting(who, "temperature", temperature, torch.float32, rows, dev, 0.0, _INF)
+    k, k_all = _setting(who, "top_k", top_k, torch.int32, rows, dev, 0, _INF)
     p, p_all = _setting(who, "top_p", top_p, torch.float32, rows, dev, 0.0, 1.0)
     m, m_all = _setting(who, "min_p", min_p, torch.float32, rows, dev, 0.0, 1.0)
     tokens = torch.empty(lead, dtype=torch.int64, device=dev)
     probs = torch.empty(lead, dtype=torch.float32, device=dev) if return_probs else None
     if rows:
-        z = logits.reshape(rows, V)
-        if z.stride(1) != 1 and V > 1 or rows > 1 and z.stride(0) < V:
-            z = z.contiguous()
-        u = uniforms.contiguous()
-        with on_device(dev):
-            _lib.check(_lib.lib().axm_sample_rows(
-                z.data_ptr(), _LOGIT_CODES[logits.dtype], z.stride(0) if rows > 1 else V, rows, V, u.data_ptr(),
-                _lib.ptr(t), _lib.ptr(k), _lib.ptr(p), _lib.ptr(m), float(t_all), min(int(k_all), V), float(p_all),
-                float(m_all), tokens.data_ptr(), _lib.ptr(probs), _lib.stream_of(dev)), who)
+        z = logits if len(shape) == 2 else logits.reshape(rows, V)
+        ld = z.stride(0) if rows > 1 else V
+        if (V > 1 and z.stride(1) != 1) or ld < V:
+            z, ld = z.contiguous(), V
+        u = uniforms if uniforms.is_contiguous() else uniforms.contiguous()
+        with on_device(dev.index):
+            rc = _lib.lib().axm_sample_rows(
+                z.data_ptr(), code, ld, rows, V, u.data_ptr(), None if t is None else t.data_ptr(),
+                None if k is None else k.data_ptr(), None if p is None else p.data_ptr(),
+                None if m is None else m.data_ptr(), t_all, min(k_all, V) if k is None else 0, p_all, m_all,
+                tokens.data_ptr(), None if probs is None else probs.data_ptr(), _lib.raw_stream(dev.index))
+        if rc:
+            _lib.check(rc, who)
     return (tokens, probs) if return_probs else tokens

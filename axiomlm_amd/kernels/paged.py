@@ -15,12 +15,14 @@ are out of range there (a page outside the pool, a sequence outside the table) a
 
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import torch
 
 from .. import _lib
-from .ops import _kv_code, on_device
+from .ops import KV_CODES, _kv_code, on_device
+
+_PAGED_KV = struct.Struct("5P2q7i4x")  # axm_paged_kv (include/axm.h)
 
 
 def _ints(who: str, name: str, t: torch.Tensor, device: torch.device, n: int) -> torch.Tensor:
@@ -29,62 +31,69 @@ def _ints(who: str, name: str, t: torch.Tensor, device: torch.device, n: int) ->
         raise ValueError(f"{who}: {name} must be an int32 or int64 tensor on {device}")
     if t.dim() != 1 or t.numel() != n:
         raise ValueError(f"{who}: {name} has shape {tuple(t.shape)}, expected ({n},)")
-    return t.to(torch.int32).contiguous()
+    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
 
-def _inside_page_contiguous(t: torch.Tensor) -> bool:
-    """Whether the last three dimensions are laid out densely (strides of dimensions of one element do not matter)."""
-    want = 1
-    for size, stride in zip(reversed(t.shape[-3:]), reversed(t.stride()[-3:])):
-        if size != 1 and stride != want:
-            return False
-        want *= size
-    return True
+def _page_stride(who: str, name: str, t: torch.Tensor) -> int:
+    """Bytes from one page to the next (the fourth last dimension); what is inside a page must be dense (strides of
+    dimensions of one element do not matter)."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 4:
+        shape, stride = shape[-4:], stride[-4:]
+    dense = shape[1] * shape[2] * shape[3]
+    if not (stride[3] == 1 and stride[2] == shape[3] and stride[1] == shape[2] * shape[3]):
+        want = 1
+        for size, step in zip(reversed(shape[1:]), reversed(stride[1:])):
+            if size != 1 and step != want:
+                raise ValueError(f"{who}: {name}'s pages must be contiguous inside")
+            want *= size
+    return (stride[0] if shape[0] > 1 else dense) * t.element_size()
 
 
-def _page_stride(t: torch.Tensor, dim: int) -> int:
-    """Bytes from one index of `dim` to the next; of a dimension of one, its dense size."""
-    n = t.stride(dim) if t.size(dim) > 1 else t[(0,) * (dim + 1)].numel()
-    return n * t.element_size()
+def _table(who: str, t: torch.Tensor, device: torch.device) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 2 or t.device != device:
+        raise ValueError(f"{who}: block_table must be a (sequences, pages) int32 tensor on {device}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _describe(who: str, k, v, ks, vs, kv_dtype: str, block_table):
-    """Checked axm_paged_kv of one layer, and the tensors that it points into."""
-    code = _kv_code(kv_dtype)
+    """Checked axm_paged_kv of one layer (packed), (B, Hkv, hd, page size, pages of a row of the table), the cache's device
+    and the table, which has to live until the call."""
+    code = KV_CODES.get(kv_dtype)
+    if code is None:
+        code = _kv_code(kv_dtype)
     for name, t in (("k_cache", k), ("v_cache", v)):
-        _lib.require_gpu(t, who)
-        if t.dim() != 4 or t.dtype not in ((torch.float16,) if code == 0 else
-                                           (torch.uint8, torch.float8_e4m3fn) if code == 1 else (torch.uint8,)):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            _lib.require_gpu(t, who)
+        if t.dim() != 4 or (t.dtype != torch.float16 if code == 0 else t.dtype != torch.uint8 and
+                            (code == 2 or t.dtype != torch.float8_e4m3fn)):
             raise ValueError(f"{who}: {name} must be (pages, n_kv_head, page_size, width) of {kv_dtype} rows, got "
                              f"{tuple(t.shape)} {t.dtype}")
-        if not _inside_page_contiguous(t):
-            raise ValueError(f"{who}: {name}'s pages must be contiguous inside")
-    if k.shape != v.shape or k.device != v.device or _page_stride(k, 0) != _page_stride(v, 0):
-        raise ValueError(f"{who}: k_cache and v_cache differ in shape, device or page stride")
-    P, Hkv, page, width = k.shape
+    shape = k.shape
+    P, Hkv, page, width = shape
+    if v.shape != shape or 0 in shape:
+        raise ValueError(f"{who}: k_cache {tuple(shape)} and v_cache {tuple(v.shape)} must be alike and not empty")
+    dev = k.device
+    stride = _page_stride(who, "k_cache", k)
+    if v.device != dev or _page_stride(who, "v_cache", v) != stride:
+        raise ValueError(f"{who}: k_cache and v_cache differ in device or page stride")
     hd = width * 2 if code == 2 else width
-    if 0 in k.shape:
-        raise ValueError(f"{who}: empty cache {tuple(k.shape)}")
     scale_stride = 0
     if code:
+        want = (P, Hkv, page, hd // 64)
         for name, t in (("k_scales", ks), ("v_scales", vs)):
             if not isinstance(t, torch.Tensor):
                 raise ValueError(f"{who}: quantized KV cache needs k_scales and v_scales")
-            if (t.dtype != torch.float16 or t.device != k.device or tuple(t.shape) != (P, Hkv, page, hd // 64)
-                    or not _inside_page_contiguous(t)):
-                raise ValueError(f"{who}: {name} must be fp16 {(P, Hkv, page, hd // 64)} on {k.device}, contiguous "
-                                 "inside a page")
-        scale_stride = _page_stride(ks, 0)
-        if scale_stride != _page_stride(vs, 0):
+            if t.dtype != torch.float16 or t.shape != want or t.device != dev:
+                raise ValueError(f"{who}: {name} must be fp16 {want} on {dev}, got {tuple(t.shape)} {t.dtype}")
+        scale_stride = _page_stride(who, "k_scales", ks)
+        if _page_stride(who, "v_scales", vs) != scale_stride:
             raise ValueError(f"{who}: k_scales and v_scales differ in page stride")
-    if (not isinstance(block_table, torch.Tensor) or block_table.device != k.device or block_table.dim() != 2
-            or block_table.dtype != torch.int32):
-        raise ValueError(f"{who}: block_table must be a (sequences, pages) int32 tensor on {k.device}")
-    table = block_table.contiguous()
+    table = _table(who, block_table, dev)
     B, max_pages = table.shape
-    d = _lib.PagedKv(k.data_ptr(), v.data_ptr(), ks.data_ptr() if code else None, vs.data_ptr() if code else None,
-                     table.data_ptr(), _page_stride(k, 0), scale_stride, code, Hkv, hd, page, P, B, max_pages)
-    return d, table
+    d = _PAGED_KV.pack(k.data_ptr(), v.data_ptr(), ks.data_ptr() if code else 0, vs.data_ptr() if code else 0,
+                       table.data_ptr(), stride, scale_stride, code, Hkv, hd, page, P, B, max_pages)
+    return d, (B, Hkv, hd, page, max_pages), dev, table
 
 
 def rope_paged_kv_cache_write(qkv: torch.Tensor, freqs_cis: torch.Tensor, k_cache: torch.Tensor,
@@ -102,35 +111,38 @@ def rope_paged_kv_cache_write(qkv: torch.Tensor, freqs_cis: torch.Tensor, k_cach
     No slot may be given twice.  freqs_cis: complex (rope_len, hd/2) or its real view (rope_len, hd/2, 2).  Rounding as
     ``rope_kv_cache_write_quantized``; FP8 codes saturate, and a group whose scale rounds to zero is stored as zeros."""
     who = "rope_paged_kv_cache_write"
-    _lib.require_gpu(qkv, who)
-    d, _table = _describe(who, k_cache, v_cache, k_scales, v_scales, kv_dtype, block_table)
-    dev = qkv.device
-    width = int(q_dim) + 2 * int(kv_dim)
-    if qkv.dtype != torch.float16 or qkv.dim() != 2 or qkv.size(1) != width or (width > 1 and qkv.stride(1) != 1):
+    d, (_, Hkv, hd, _, _), dev, table = _describe(who, k_cache, v_cache, k_scales, v_scales, kv_dtype, block_table)
+    width = q_dim + 2 * kv_dim
+    if not isinstance(qkv, torch.Tensor) or qkv.device != dev:
+        _lib.require_gpu(qkv, who)
+        raise ValueError(f"{who}: qkv is on {qkv.device}, the cache on {dev}")
+    if qkv.dtype != torch.float16 or qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1:
         raise ValueError(f"{who}: qkv must be fp16 (tokens, q_dim + 2 kv_dim = {width}) with contiguous rows, got "
                          f"{tuple(qkv.shape)} {qkv.dtype}")
-    if dev != k_cache.device:
-        raise ValueError(f"{who}: qkv is on {dev}, the cache on {k_cache.device}")
-    if head_dim != d.head_dim or kv_dim != d.n_kv_head * d.head_dim:
-        raise ValueError(f"{who}: kv_dim {kv_dim} of heads of {head_dim} does not match the cache's {d.n_kv_head} heads "
-                         f"of {d.head_dim}")
-    T = qkv.size(0)
+    if head_dim != hd or kv_dim != Hkv * hd:
+        raise ValueError(f"{who}: kv_dim {kv_dim} of heads of {head_dim} does not match the cache's {Hkv} heads of {hd}")
+    T = qkv.shape[0]
     if T == 0:
         return
     pos = _ints(who, "positions", positions, dev, T)
     sl = None if slots is None else _ints(who, "slots", slots, dev, T)
     seq = None if seq_ids is None else _ints(who, "seq_ids", seq_ids, dev, T)
     fr = torch.view_as_real(freqs_cis) if freqs_cis.is_complex() else freqs_cis
-    fr = fr.to(device=dev, dtype=torch.float32).contiguous()
-    if fr.dim() != 3 or fr.size(0) < 1 or tuple(fr.shape[1:]) != (head_dim // 2, 2):
+    if fr.dtype != torch.float32 or fr.device != dev or not fr.is_contiguous():
+        fr = fr.to(device=dev, dtype=torch.float32).contiguous()
+    shape = fr.shape
+    if len(shape) != 3 or shape[0] < 1 or shape[1] * 2 != hd or shape[2] != 2:
         raise ValueError(f"{who}: freqs_cis of shape {tuple(freqs_cis.shape)} for heads of {head_dim}")
     bias = None if qkv_bias is None else qkv_bias.to(device=dev, dtype=torch.float16).contiguous()
     if bias is not None and bias.numel() != width:
         raise ValueError(f"{who}: qkv_bias has {bias.numel()} elements, expected {width}")
-    with on_device(dev):
-        _lib.check(_lib.lib().axm_rope_paged_kv_write(
-            qkv.data_ptr(), qkv.stride(0) if T > 1 else width, T, fr.data_ptr(), fr.size(0), pos.data_ptr(),
-            _lib.ptr(sl), _lib.ptr(seq), _lib.ptr(bias), ctypes.byref(d), int(q_dim), _lib.stream_of(dev)), who)
+    with on_device(dev.index):
+        rc = _lib.lib().axm_rope_paged_kv_write(
+            qkv.data_ptr(), qkv.stride(0) if T > 1 else width, T, fr.data_ptr(), shape[0], pos.data_ptr(),
+            None if sl is None else sl.data_ptr(), None if seq is None else seq.data_ptr(),
+            None if bias is None else bias.data_ptr(), d, q_dim, _lib.raw_stream(dev.index))
+    if rc:
+        _lib.check(rc, who)
 
 
 def gqa_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -144,44 +156,43 @@ def gqa_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     mass (fp32 (B, Hkv, M), M >= max_pages * page_size, contiguous): the softmax weights of every slot, summed over the
     query heads of the KV head, are added to it: the account that ``evict_paged_kv`` goes by."""
     who = "gqa_paged_decode"
-    _lib.require_gpu(q, who)
-    d, _table = _describe(who, k_cache, v_cache, k_scales, v_scales, kv_dtype, block_table)
-    dev, hd = q.device, d.head_dim
-    if q.dim() not in (3, 4) or (q.dim() == 4 and q.size(2) != 1) or q.size(0) != d.n_seqs or q.size(-1) != hd:
-        raise ValueError(f"{who}: q of shape {tuple(q.shape)} for {d.n_seqs} sequences and heads of {hd}")
-    Hq = q.size(1)
-    if dev != k_cache.device:
-        raise ValueError(f"{who}: q is on {dev}, the cache on {k_cache.device}")
-    if Hq < 1 or Hq % d.n_kv_head or Hq // d.n_kv_head > 64:
-        raise ValueError(f"{who}: {Hq} query heads for {d.n_kv_head} KV heads")
-    lens = _ints(who, "seq_lens", seq_lens, dev, d.n_seqs)
-    out = torch.empty(q.shape, dtype=torch.float16, device=dev)
-    if d.n_seqs == 0:
+    d, (B, Hkv, hd, page, max_pages), dev, table = _describe(who, k_cache, v_cache, k_scales, v_scales, kv_dtype,
+                                                             block_table)
+    if not isinstance(q, torch.Tensor) or q.device != dev:
+        _lib.require_gpu(q, who)
+        raise ValueError(f"{who}: q is on {q.device}, the cache on {dev}")
+    shape = q.shape
+    if len(shape) not in (3, 4) or (len(shape) == 4 and shape[2] != 1) or shape[0] != B or shape[-1] != hd:
+        raise ValueError(f"{who}: q of shape {tuple(shape)} for {B} sequences and heads of {hd}")
+    Hq = shape[1]
+    if Hq < 1 or Hq % Hkv or Hq // Hkv > 64:
+        raise ValueError(f"{who}: {Hq} query heads for {Hkv} KV heads")
+    lens = _ints(who, "seq_lens", seq_lens, dev, B)
+    out = torch.empty(shape, dtype=torch.float16, device=dev)
+    if B == 0:
         return out
-    if d.max_pages == 0:
+    if max_pages == 0:
         return out.zero_()
     M = 0
     if mass is not None:
-        M = mass.size(-1) if isinstance(mass, torch.Tensor) and mass.dim() == 3 else -1
-        if (M < d.max_pages * d.page_size or tuple(mass.shape[:2]) != (d.n_seqs, d.n_kv_head)
-                or mass.dtype != torch.float32 or mass.device != dev or not mass.is_contiguous()):
-            raise ValueError(f"{who}: mass must be contiguous fp32 ({d.n_seqs}, {d.n_kv_head}, at least "
-                             f"{d.max_pages * d.page_size}) on {dev}")
-    qc = q.to(torch.float16)
-    ld = qc.stride(0)
-    if qc.stride(-1) != 1 or (Hq > 1 and qc.stride(1) != hd) or qc.data_ptr() % 16 or (d.n_seqs > 1 and ld % 8) \
-            or (d.n_seqs > 1 and ld < Hq * hd):
-        qc = qc.contiguous()
-        if qc.data_ptr() % 16:
-            qc = qc.clone()
-    ld = qc.stride(0) if d.n_seqs > 1 else Hq * hd
-    with on_device(dev):
+        M = mass.shape[2] if isinstance(mass, torch.Tensor) and mass.dim() == 3 else -1
+        if (M < max_pages * page or mass.shape[0] != B or mass.shape[1] != Hkv or mass.dtype != torch.float32
+                or mass.device != dev or not mass.is_contiguous()):
+            raise ValueError(f"{who}: mass must be contiguous fp32 ({B}, {Hkv}, at least {max_pages * page}) on {dev}")
+    qc = q if q.dtype == torch.float16 else q.to(torch.float16)
+    stride = qc.stride()
+    ld = stride[0] if B > 1 else Hq * hd
+    if stride[-1] != 1 or (Hq > 1 and stride[1] != hd) or ld % 8 or ld < Hq * hd or qc.data_ptr() % 16:
+        qc, ld = qc.clone(memory_format=torch.contiguous_format), Hq * hd
+    with on_device(dev.index):
         L = _lib.lib()
-        need = L.axm_paged_decode_workspace_bytes(d.n_seqs, Hq, d.n_kv_head, hd, d.page_size, d.max_pages,
-                                                  mass is not None)
+        need = L.axm_paged_decode_workspace_bytes(B, Hq, Hkv, hd, page, max_pages, 0 if mass is None else 1)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _lib.check(L.axm_paged_flash_decode(qc.data_ptr(), ld, ctypes.byref(d), lens.data_ptr(), out.data_ptr(), Hq,
-                                            _lib.ptr(mass), M, _lib.ptr(ws), need, _lib.stream_of(dev)), who)
+        rc = L.axm_paged_flash_decode(qc.data_ptr(), ld, d, lens.data_ptr(), out.data_ptr(), Hq,
+                                      None if mass is None else mass.data_ptr(), M,
+                                      None if ws is None else ws.data_ptr(), need, _lib.raw_stream(dev.index))
+    if rc:
+        _lib.check(rc, who)
     return out
 
 
@@ -198,41 +209,53 @@ def evict_paged_kv(cache: torch.Tensor, scales: torch.Tensor | None, block_table
     Keys stay rotated at the positions they had: the next token's position goes on counting, its slot is the new length.
     The pages of a sequence over the budget must belong to it alone."""
     who = "evict_paged_kv"
-    _lib.require_gpu(cache, who)
-    if cache.dim() != 6 or cache.size(1) != 2:
-        raise ValueError(f"{who}: cache must be (layers, 2, pages, n_kv_head, page_size, width), got "
-                         f"{tuple(cache.shape)}")
-    if cache.dtype == torch.float16:
-        kv_dtype = "fp16"
-    elif not isinstance(scales, torch.Tensor) or scales.dim() != 6 or scales.shape[:5] != cache.shape[:5]:
-        raise ValueError(f"{who}: quantized KV cache needs scales (layers, 2, pages, n_kv_head, page_size, hd / 64)")
-    else:
-        kv_dtype = "fp8" if scales.size(5) * 64 == cache.size(5) else "int4"
-    L = cache.size(0)
-    if L < 1:
-        raise ValueError(f"{who}: cache without layers")
-    quant = kv_dtype != "fp16"
-    d, table = _describe(who, cache[0, 0], cache[0, 1], scales[0, 0] if quant else None,
-                         scales[0, 1] if quant else None, kv_dtype, block_table)
-    dev, B, H = cache.device, d.n_seqs, d.n_kv_head
+    if not isinstance(cache, torch.Tensor) or not cache.is_cuda:
+        _lib.require_gpu(cache, who)
+    shape = cache.shape
+    if len(shape) != 6 or shape[1] != 2 or shape[0] < 1:
+        raise ValueError(f"{who}: cache must be (layers, 2, pages, n_kv_head, page_size, width), got {tuple(shape)}")
+    dev = cache.device
+    L, _, P, H, page, width = shape
+    quant = cache.dtype != torch.float16
+    code, hd, item = 0, width, 2
+    stride, scale_stride = cache.stride(), (0, 0)
+    scale_page, scale_ptr = 0, 0
+    if quant:
+        groups = scales.shape[5] if isinstance(scales, torch.Tensor) and scales.dim() == 6 else 0
+        code, hd, item = (1, width, 1) if groups * 64 == width else (2, 2 * width, 1)
+        if (cache.dtype not in (torch.uint8, torch.float8_e4m3fn) or not groups or groups * 64 != hd
+                or scales.shape[:5] != shape[:5] or scales.dtype != torch.float16 or scales.device != dev):
+            raise ValueError(f"{who}: quantized KV cache (uint8 codes) needs fp16 scales (layers, 2, pages, n_kv_head, "
+                             "page_size, hd / 64)")
+        scale_stride, scale_page, scale_ptr = scales.stride(), _page_stride(who, "scales", scales), scales.data_ptr()
+    if 0 in shape:
+        raise ValueError(f"{who}: empty cache {tuple(shape)}")
+    table = _table(who, block_table, dev)
+    B, max_pages = table.shape
+    ptr = cache.data_ptr()
+    d = _PAGED_KV.pack(ptr, ptr + stride[1] * item, scale_ptr, scale_ptr + scale_stride[1] * 2, table.data_ptr(),
+                       _page_stride(who, "cache", cache), scale_page, code, H, hd, page, P, B, max_pages)
     budget, recent = int(budget), int(recent)
     if budget < 1 or not 0 <= recent <= budget:
         raise ValueError(f"{who}: budget {budget} must be positive and recent {recent} within it")
     if (not isinstance(mass, torch.Tensor) or mass.dtype != torch.float32 or mass.device != dev or mass.dim() != 4
-            or tuple(mass.shape[:3]) != (L, B, H) or mass.size(3) < d.max_pages * d.page_size):
-        raise ValueError(f"{who}: mass must be fp32 ({L}, {B}, {H}, at least {d.max_pages * d.page_size}) on {dev}")
+            or mass.shape[:3] != (L, B, H) or mass.shape[3] < max_pages * page):
+        raise ValueError(f"{who}: mass must be fp32 ({L}, {B}, {H}, at least {max_pages * page}) on {dev}")
     lens = _ints(who, "seq_lens", seq_lens, dev, B)
-    mass = mass.contiguous()
+    if not mass.is_contiguous():
+        mass = mass.contiguous()
     kept = torch.empty((L, B, H, budget), dtype=torch.int32, device=dev)
     out_lens = torch.empty(B, dtype=torch.int32, device=dev)
-    out_mass = torch.empty_like(mass)
+    out_mass = torch.empty(mass.shape, dtype=torch.float32, device=dev)
     if B == 0:
         return kept, out_lens, out_mass
-    if d.max_pages == 0:
+    if max_pages == 0:
         return kept.fill_(-1), out_lens.zero_(), out_mass.zero_()
-    with on_device(dev):
-        _lib.check(_lib.lib().axm_evict_paged_kv(
-            ctypes.byref(d), L, _page_stride(cache, 0), _page_stride(scales, 0) if quant else 0, lens.data_ptr(),
-            mass.data_ptr(), mass.size(3), budget, recent, out_mass.data_ptr(), kept.data_ptr(), out_lens.data_ptr(),
-            _lib.stream_of(dev)), who)
+    with on_device(dev.index):
+        rc = _lib.lib().axm_evict_paged_kv(
+            d, L, stride[0] * item, scale_stride[0] * 2, lens.data_ptr(),
+            mass.data_ptr(), mass.shape[3], budget, recent, out_mass.data_ptr(), kept.data_ptr(), out_lens.data_ptr(),
+            _lib.raw_stream(dev.index))
+    if rc:
+        _lib.check(rc, who)
     return kept, out_lens, out_mass
