@@ -22,6 +22,7 @@ from torch import Tensor
 from torch.library import custom_op
 
 from .kernels import ops as _ops
+from .kernels import paged as _paged
 from .kernels import quant as _q
 
 
@@ -200,3 +201,53 @@ def argmax_rows(logits: Tensor) -> Tensor:
 @argmax_rows.register_fake
 def _(logits):
     return logits.new_empty(logits.shape[:-1], dtype=torch.int64)
+
+
+# ---------------------------------------------------------------------------
+# Paged KV cache and sampling (no counterpart in the reference's module)
+# ---------------------------------------------------------------------------
+@custom_op("axiomlm::rope_paged_kv_cache_write", mutates_args=("qkv", "k_cache", "v_cache", "k_scales", "v_scales"))
+def rope_paged_kv_cache_write(qkv: Tensor, freqs_cis: Tensor, k_cache: Tensor, v_cache: Tensor,
+                              k_scales: Optional[Tensor], v_scales: Optional[Tensor], block_table: Tensor,
+                              positions: Tensor, q_dim: int, kv_dim: int, head_dim: int,
+                              slots: Optional[Tensor] = None, seq_ids: Optional[Tensor] = None,
+                              qkv_bias: Optional[Tensor] = None, kv_dtype: str = "fp16") -> None:
+    _paged.rope_paged_kv_cache_write(qkv, freqs_cis, k_cache, v_cache, block_table, positions, q_dim, kv_dim, head_dim,
+                                     slots, seq_ids, qkv_bias, k_scales, v_scales, kv_dtype)
+
+
+@custom_op("axiomlm::gqa_paged_decode", mutates_args=("mass",))
+def gqa_paged_decode(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, seq_lens: Tensor,
+                     k_scales: Optional[Tensor] = None, v_scales: Optional[Tensor] = None, kv_dtype: str = "fp16",
+                     mass: Optional[Tensor] = None) -> Tensor:
+    return _paged.gqa_paged_decode(q, k_cache, v_cache, block_table, seq_lens, k_scales, v_scales, kv_dtype, mass)
+
+
+@gqa_paged_decode.register_fake
+def _(q, k_cache, v_cache, block_table, seq_lens, k_scales=None, v_scales=None, kv_dtype="fp16", mass=None):
+    return q.new_empty(q.shape, dtype=torch.float16)
+
+
+@custom_op("axiomlm::evict_paged_kv", mutates_args=("cache", "scales"))
+def evict_paged_kv(cache: Tensor, scales: Optional[Tensor], block_table: Tensor, seq_lens: Tensor, mass: Tensor,
+                   budget: int, recent: int) -> tuple[Tensor, Tensor, Tensor]:
+    return _paged.evict_paged_kv(cache, scales, block_table, seq_lens, mass, budget, recent)
+
+
+@evict_paged_kv.register_fake
+def _(cache, scales, block_table, seq_lens, mass, budget, recent):
+    return (mass.new_empty((*mass.shape[:3], budget), dtype=torch.int32),
+            seq_lens.new_empty(seq_lens.shape, dtype=torch.int32), mass.new_empty(mass.shape))
+
+
+@custom_op("axiomlm::sample_tokens", mutates_args=())
+def sample_tokens(logits: Tensor, uniforms: Tensor, temperature: Tensor, top_k: Tensor, top_p: Tensor,
+                  min_p: Tensor) -> tuple[Tensor, Tensor]:
+    """Tokens and their probabilities; every setting a tensor of one per row (or of none: 0-d, on the host)."""
+    return _ops.sample_tokens(logits, uniforms, temperature, top_k, top_p, min_p, return_probs=True)
+
+
+@sample_tokens.register_fake
+def _(logits, uniforms, temperature, top_k, top_p, min_p):
+    lead = logits.shape[:-1]
+    return logits.new_empty(lead, dtype=torch.int64), logits.new_empty(lead, dtype=torch.float32)
