@@ -400,14 +400,14 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
     k, k_all = _setting(who, "top_k", top_k, torch.int32, rows, dev, 0, _INF)
     p, p_all = _setting(who, "top_p", top_p, torch.float32, rows, dev, 0.0, 1.0)
     m, m_all = _setting(who, "min_p", min_p, torch.float32, rows, dev, 0.0, 1.0)
-    tokens = torch.empty(lead, dtype=torch.int64, device=dev)
-    probs = torch.empty(lead, dtype=torch.float32, device=dev) if return_probs else None
+    u = uniforms if uniforms.shape == lead and uniforms.is_contiguous() else uniforms.reshape(lead).contiguous()
+    tokens = torch.empty_like(u, dtype=torch.int64)
+    probs = torch.empty_like(u) if return_probs else None
     if rows:
         z = logits if len(shape) == 2 else logits.reshape(rows, V)
         ld = z.stride(0) if rows > 1 else V
         if (V > 1 and z.stride(1) != 1) or ld < V:
             z, ld = z.contiguous(), V
-        u = uniforms if uniforms.is_contiguous() else uniforms.contiguous()
         with on_device(dev.index):
             rc = _lib.lib().axm_sample_rows(
                 z.data_ptr(), code, ld, rows, V, u.data_ptr(), None if t is None else t.data_ptr(),

@@ -168,7 +168,7 @@ def gqa_paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if Hq < 1 or Hq % Hkv or Hq // Hkv > 64:
         raise ValueError(f"{who}: {Hq} query heads for {Hkv} KV heads")
     lens = _ints(who, "seq_lens", seq_lens, dev, B)
-    out = torch.empty(shape, dtype=torch.float16, device=dev)
+    out = torch.empty_like(q, dtype=torch.float16, memory_format=torch.contiguous_format)
     if B == 0:
         return out
     if max_pages == 0:
@@ -245,8 +245,7 @@ def evict_paged_kv(cache: torch.Tensor, scales: torch.Tensor | None, block_table
     if not mass.is_contiguous():
         mass = mass.contiguous()
     kept = torch.empty((L, B, H, budget), dtype=torch.int32, device=dev)
-    out_lens = torch.empty(B, dtype=torch.int32, device=dev)
-    out_mass = torch.empty(mass.shape, dtype=torch.float32, device=dev)
+    out_lens, out_mass = torch.empty_like(lens), torch.empty_like(mass)
     if B == 0:
         return kept, out_lens, out_mass
     if max_pages == 0:
