@@ -133,8 +133,9 @@ _SIGNATURES = {
     "axm_sample_rows": (
         c_int,
         [c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_int,
-         c_float, c_float, c_void_p, c_void_p, c_void_p],
+         c_float, c_float, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
     ),
+    "axm_sample_rows_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "axm_runner_create": (c_int, [c_void_p, c_void_p]),
     "axm_runner_destroy": (None, [c_void_p]),
     "axm_runner_step": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_void_p]),

@@ -18,10 +18,7 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 2048;
 constexpr float kBinsPerUnit = 64.f;
 constexpr int kList = 2048;  // candidates in LDS
-#ifndef AH
-#define AH 2
-#endif
-constexpr int kAhead = AH;
+constexpr int kAhead = 2;    // loads of a wave under way
 constexpr int kSums = 3072;  // entries of the running sum
 
 // 2^(j / 64), rounded to nearest.
@@ -57,6 +54,24 @@ struct SampleParams {
   int top_k_all;
   int64_t* tokens;
   float* probs;
+  // Few rows: `slices` workgroups share a row without top-k (SplitRow); 0: none do.
+  int slices;
+  struct SliceTop* tops;  // [rows][slices]
+  uint64_t* hists;        // [rows][slices][kBins]
+  uint64_t* sums;         // [rows][kSums]
+  uint64_t* lists;        // [rows][slices][kList]
+  struct SplitRow* split; // [rows]
+};
+
+struct SliceTop {
+  float top;
+  int octave;  // the slice's weights are 2^shift 2^(z log2(e) / T - octave)
+  int listed;  // candidates of the bin with the cut (second launch)
+};
+struct SplitRow {  // what the second launch found
+  double need;
+  uint64_t ahead;
+  int bin;
 };
 
 // Order of logits as integers (finite values and +inf; -0 counts as 0).
@@ -256,6 +271,9 @@ struct Row {
   }
 };
 
+constexpr double kRate = 64.0 * 1.4426950408889634;
+// Tiles of an entry of the running sum.
+__device__ __forceinline__ int tile_group(int vectors) { return ((vectors + 63) / 64 + kSums - 1) / kSums; }
 __device__ __forceinline__ int bin_of(float top, float z) {  // -inf and NaN: the last
   return (int)fminf((top - z) * kBinsPerUnit, (float)(kBins - 1));
 }
@@ -264,11 +282,11 @@ __device__ __forceinline__ int bin_of(float top, float z) {  // -inf and NaN: th
 // 2^-7 octaves either way (four terms: 2^-44 of the weight), rounded by adding 2^52.  z - top and what follows in 64
 // bits: differences of fp32 logits do not fit 32.
 struct Weight {
-  double top, rate;  // rate: 64 log2(e) / T
+  double top, rate, off;  // rate: 64 log2(e) / T; off: added in 64ths of an octave
   int shift;
   const double* table;
   __device__ __forceinline__ uint64_t operator()(float z) const {
-    const double y = fmax(((double)z - top) * rate, -64.0 * 1024.0);
+    const double y = fmax(fma((double)z - top, rate, off), -64.0 * 1024.0);
     const double near = y + 6755399441055744.0;  // 1.5 2^52: the nearest integer in the low bits
     const int i = (int)(uint32_t)__builtin_bit_cast(uint64_t, near);
     const double r = y - (near - 6755399441055744.0);
@@ -279,15 +297,11 @@ struct Weight {
   }
 };
 
-// The first logit, in index order, at which the running sum of weights passes `target` (sums compared as doubles), or the
-// last one with a weight.  -> its index in s.where, its weight in s.before, all weights' sum in s.total.
-// f(tile, z, add) calls add(j, weight) for the tile's logits that have one; frac >= 0: target is that share of the sum.
+// Sums of the weights of every `group` tiles, in s.sums; f(tile, z, add) calls add(j, weight) for the tile's logits that
+// have one.
 template <int DT, typename F>
-__device__ __forceinline__ void find_in_order(const Row<DT>& row, Lds& s, int& turn, const F& f, double frac,
-                                              double target) {
+__device__ __forceinline__ void sum_tiles(const Row<DT>& row, Lds& s, int group, const F& f) {
   constexpr int E = Row<DT>::E;
-  const int lane = threadIdx.x & 63;
-  const int tiles = (row.vectors + 63) / 64, group = (tiles + kSums - 1) / kSums;
   __syncthreads();
   for (int i = threadIdx.x; i < kSums; i += kThreads) s.sums[i] = 0;
   __syncthreads();
@@ -296,10 +310,20 @@ __device__ __forceinline__ void find_in_order(const Row<DT>& row, Lds& s, int& t
     f(tile, z, [&](int, uint64_t x) { w += x; });
     if (__builtin_amdgcn_ballot_w64(w != 0)) {
       w = wave_prefix64(w);
-      if (lane == 63) atomicAdd((unsigned long long*)&s.sums[tile / group], (unsigned long long)w);
+      if ((threadIdx.x & 63) == 63) atomicAdd((unsigned long long*)&s.sums[tile / group], (unsigned long long)w);
     }
   });
   __syncthreads();
+}
+
+// The first logit, in index order, at which the running sum of weights (s.sums, and f within a group) passes `target`
+// (sums compared as doubles), or the last one with a weight.  -> its index in s.where, its weight in s.before, all
+// weights' sum in s.total.  frac >= 0: target is that share of the sum.
+template <int DT, typename F>
+__device__ __forceinline__ void pick_in_order(const Row<DT>& row, Lds& s, int& turn, int group, const F& f, double frac,
+                                              double target) {
+  constexpr int E = Row<DT>::E;
+  const int tiles = (row.vectors + 63) / 64;
   constexpr int kEach = kSums / kThreads;
   uint64_t e[kEach], mine = 0, total;
 #pragma unroll
@@ -350,25 +374,212 @@ __device__ __forceinline__ void find_in_order(const Row<DT>& row, Lds& s, int& t
   __syncthreads();
 }
 
+template <int DT, typename F>
+__device__ __forceinline__ void find_in_order(const Row<DT>& row, Lds& s, int& turn, const F& f, double frac,
+                                              double target) {
+  const int group = tile_group(row.vectors);
+  sum_tiles<DT>(row, s, group, f);
+  pick_in_order<DT>(row, s, turn, group, f, frac, target);
+}
+
+struct Settings {
+  float temperature, top_p, min_p;
+  int k;  // 0: off
+  bool greedy;
+};
+__device__ __forceinline__ Settings settings_of(const SampleParams& p, int r) {
+  Settings t;
+  t.temperature = p.temperature ? p.temperature[r] : p.temperature_all;
+  const int k = p.top_k ? p.top_k[r] : p.top_k_all;
+  t.k = k > 0 && k < p.V ? k : 0;
+  t.top_p = p.top_p ? p.top_p[r] : p.top_p_all;
+  t.min_p = p.min_p ? p.min_p[r] : p.min_p_all;
+  t.greedy = !(t.temperature > 0.f);
+  return t;
+}
+
+// Row r, with the tiles [tile0, tile1) of a workgroup dealt to its waves in contiguous runs.
 template <int DT>
-__global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
+__device__ __forceinline__ Row<DT> row_of(const SampleParams& p, int r) {
   constexpr int E = Row<DT>::E, kSize = DT == 1 ? 4 : 2;
-  __shared__ Lds s;
-  const int r = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uintptr_t first = (uintptr_t)p.logits + (uintptr_t)((int64_t)r * p.ld * kSize);
   Row<DT> row;
   row.base = (const u32x4*)(first & ~(uintptr_t)15);
   row.lead = (int)(first & 15) / kSize;
   row.V = p.V;
   row.vectors = (row.lead + p.V + E - 1) / E;
-  const int tiles = (row.vectors + 63) / 64;
-  row.tile0 = (int)((int64_t)tiles * wave / kWaves);
-  row.tile1 = (int)((int64_t)tiles * (wave + 1) / kWaves);
   row.inf = false;
-  const float temperature = p.temperature ? p.temperature[r] : p.temperature_all;
-  const int top_k = p.top_k ? p.top_k[r] : p.top_k_all;
-  const float top_p = p.top_p ? p.top_p[r] : p.top_p_all;
-  const float min_p = p.min_p ? p.min_p[r] : p.min_p_all;
+  return row;
+}
+template <int DT>
+__device__ __forceinline__ void deal_tiles(Row<DT>& row, int tile0, int tile1) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  row.tile0 = tile0 + (int)((int64_t)(tile1 - tile0) * wave / kWaves);
+  row.tile1 = tile0 + (int)((int64_t)(tile1 - tile0) * (wave + 1) / kWaves);
+  if (row.tile0 < row.tile1) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) row.first[k] = row.load(min(row.tile0 + k, row.tile1 - 1));
+  }
+}
+// Slice `slice` of a row: whole groups of tiles.
+template <int DT>
+__device__ __forceinline__ void deal_slice(Row<DT>& row, int slice, int slices) {
+  const int group = tile_group(row.vectors), tiles = (row.vectors + 63) / 64, groups = (tiles + group - 1) / group;
+  deal_tiles<DT>(row, min((int)((int64_t)groups * slice / slices) * group, tiles),
+                 min((int)((int64_t)groups * (slice + 1) / slices) * group, tiles));
+}
+
+// ---------------------------------------------------------------------------
+// Few rows of large vocabularies, without top-k: `slices` workgroups a row.  First launch: every slice's largest logit and
+// its histogram of weights, over bins of a grid that all slices share (floor(64 z)) and relative to an octave of its
+// own; second: every slice adds the histograms up (shifted by whole bins and octaves), finds the bin with the cut, sums
+// its tiles' weights before that bin and lists the bin's candidates; third: one workgroup a row cuts the list, adds what
+// stays to the sums and picks the token.  Rows whose largest logit is infinite or passes 2^17 or 2^20 octaves,
+// and those that list too many, are left to the third launch, which then does everything.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float grid_of(float z) { return floorf(z * kBinsPerUnit); }
+__device__ __forceinline__ int grid_bin(float top_grid, float z) {
+  return (int)fminf(top_grid - grid_of(z), (float)(kBins - 1));
+}
+// Weights of a split row: relative to whole octaves.
+__device__ __forceinline__ Weight octave_weight(float temperature, int octave, int shift, const double* table) {
+  return Weight{0.0, kRate / (double)temperature, -64.0 * (double)octave, shift, table};
+}
+// The row's largest logit and octave from its slices'; false: not to be split.
+__device__ __forceinline__ bool split_top(const SampleParams& p, int r, float* top, int* octave) {
+  float t = -INFINITY;
+  int o = -(1 << 30);
+  for (int i = 0; i < p.slices; ++i) {
+    const SliceTop x = p.tops[(int64_t)r * p.slices + i];
+    if (x.top > t) t = x.top;
+    o = max(o, x.octave);
+  }
+  *top = t;
+  *octave = o;
+  return fabsf(t) < 131072.f && abs(o) < (1 << 20);  // (bins of larger logits are not whole in fp32)
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads) sample_slice_kernel(SampleParams p) {
+  constexpr int E = Row<DT>::E;
+  __shared__ Lds s;
+  const int r = blockIdx.x / p.slices, slice = blockIdx.x % p.slices;
+  const Settings t = settings_of(p, r);
+  if (t.greedy || t.k > 0) return;
+  Row<DT> row = row_of<DT>(p, r);
+  deal_slice<DT>(row, slice, p.slices);
+  int turn = 0;
+  if (threadIdx.x < 64) s.table[threadIdx.x] = kOctave[threadIdx.x];
+  for (int i = threadIdx.x; i < kBins; i += kThreads) s.bins.weight[i] = 0;
+  float top = -INFINITY;
+  row.pass([&](int, const float (&z)[E]) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) top = fmaxf(top, z[j]);
+  });
+  const uint32_t best = (uint32_t)block_max(top > -INFINITY ? order_key(top) : 0, s, turn);
+  top = best ? key_value(best) : -INFINITY;
+  const double octave = ceil((double)top * (kRate / 64.0) / (double)t.temperature);
+  const bool fine = best && fabs(octave) < (double)(1 << 20);
+  if (threadIdx.x == 0)
+    p.tops[blockIdx.x] = SliceTop{top, fine ? (int)octave : !best || octave < 0.0 ? -(1 << 30) : 1 << 30, 0};
+  if (!fine || !(t.top_p < 1.f)) return;
+  const Weight weight = octave_weight(t.temperature, (int)octave, p.shift, s.table);
+  const float top_grid = grid_of(top);
+  row.pass([&](int, const float (&z)[E]) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const uint64_t w = weight(z[j]);  // (of all: eight chains side by side)
+      if (z[j] > -INFINITY) atomicAdd((unsigned long long*)&s.bins.weight[grid_bin(top_grid, z[j])], (unsigned long long)w);
+    }
+  });
+  __syncthreads();
+  uint64_t* to = p.hists + (int64_t)blockIdx.x * kBins;
+  for (int i = threadIdx.x; i < kBins; i += kThreads) to[i] = s.bins.weight[i];
+}
+
+// min-p of a split row: the least weight that stays.
+__device__ __forceinline__ uint64_t least_of(float min_p, uint64_t largest) {
+  return (uint64_t)fmin(fmax(ceil((double)min_p * (double)largest), 0.0), (double)largest);
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads) sample_sums_kernel(SampleParams p) {
+  constexpr int E = Row<DT>::E;
+  __shared__ Lds s;
+  const int r = blockIdx.x / p.slices, slice = blockIdx.x % p.slices;
+  const Settings t = settings_of(p, r);
+  if (t.greedy || t.k > 0) return;
+  float top;
+  int octave, turn = 0;
+  if (!split_top(p, r, &top, &octave)) return;
+  Row<DT> row = row_of<DT>(p, r);
+  deal_slice<DT>(row, slice, p.slices);
+  if (threadIdx.x < 64) s.table[threadIdx.x] = kOctave[threadIdx.x];
+  for (int i = threadIdx.x; i < kBins; i += kThreads) s.bins.weight[i] = 0;
+  if (threadIdx.x == 0) s.n = 0, s.bin = 0, s.before = 0;
+  __syncthreads();
+  const float top_grid = grid_of(top);
+  int bin = kBins;  // the bin with the cut; past the last: no top-p
+  if (t.top_p < 1.f) {
+    for (int i = 0; i < p.slices; ++i) {
+      const SliceTop x = p.tops[(int64_t)r * p.slices + i];
+      const int down = octave - x.octave;
+      if (x.top == -INFINITY || down > 63) continue;
+      const int by = (int)fminf(top_grid - grid_of(x.top), (float)kBins);
+      const uint64_t* from = p.hists + ((int64_t)r * p.slices + i) * kBins;
+#pragma unroll
+      for (int e = 0; e < kBins / kThreads; ++e) {
+        const int b = e * kThreads + threadIdx.x;
+        const uint64_t w = from[b] >> down;
+        if (w != 0) atomicAdd((unsigned long long*)&s.bins.weight[min(b + by, kBins - 1)], (unsigned long long)w);
+      }
+    }
+    __syncthreads();
+    uint64_t all;
+    const uint64_t c0 = s.bins.weight[2 * threadIdx.x], c1 = s.bins.weight[2 * threadIdx.x + 1];
+    const uint64_t before = block_before(c0 + c1, s, turn, &all);
+    const double need = (double)t.top_p * (double)all;
+    if ((double)before < need && (double)(before + c0 + c1) >= need) {
+      const bool second = (double)(before + c0) < need;
+      s.bin = 2 * threadIdx.x + second;
+      s.before = before + (second ? c0 : 0);
+    }
+    __syncthreads();
+    bin = s.bin;
+    if (slice == 0 && threadIdx.x == 0) p.split[r] = SplitRow{need, s.before, bin};
+  }
+  const Weight weight = octave_weight(t.temperature, octave, p.shift, s.table);
+  const uint64_t least = least_of(t.min_p, weight(top));
+  uint64_t* list = p.lists + (int64_t)blockIdx.x * kList;
+  const int group = tile_group(row.vectors);
+  sum_tiles<DT>(row, s, group, [&](int tile, const float (&z)[E], auto add) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const uint64_t w = weight(z[j]);
+      const int b = grid_bin(top_grid, z[j]);
+      add(j, (z[j] > -INFINITY) & (b < bin) & (w >= least) ? w : 0);
+      if (b == bin && z[j] > -INFINITY) {
+        const int at = atomicAdd(&s.n, 1);
+        if (at < kList) list[at] = candidate(z[j], row.index(tile, j));
+      }
+    }
+  });
+  if (threadIdx.x == 0) p.tops[blockIdx.x].listed = s.n;
+  const int tiles = (row.vectors + 63) / 64, groups = (tiles + group - 1) / group;
+  const int g0 = (int)((int64_t)groups * slice / p.slices), g1 = (int)((int64_t)groups * (slice + 1) / p.slices);
+  for (int i = g0 + threadIdx.x; i < g1; i += kThreads) p.sums[(int64_t)r * kSums + i] = s.sums[i];
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
+  constexpr int E = Row<DT>::E;
+  __shared__ Lds s;
+  const int r = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Row<DT> row = row_of<DT>(p, r);
+  const Settings settings = settings_of(p, r);
+  const float temperature = settings.temperature, top_p = settings.top_p, min_p = settings.min_p;
+  const bool greedy = settings.greedy;
+  const int k = settings.k;
   const double u = fmin(fmax((double)p.u[r], 0.0), 1.0);  // (NaN: 0)
 
   int turn = 0;
@@ -376,12 +587,65 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
     p.tokens[r] = token;
     if (p.probs) p.probs[r] = prob;
   };
-  if (row.tile0 < row.tile1) {
+  float split_z;
+  int octave;
+  if (p.slices > 0 && !greedy && k == 0 && split_top(p, r, &split_z, &octave)) {
+    // The slices have summed what lies before the bin with the cut and listed the bin.
+    int n = 0;
+    for (int i = 0; i < p.slices; ++i) n += p.tops[(int64_t)r * p.slices + i].listed;
+    if (n <= kList) {
+      if (threadIdx.x < 64) s.table[threadIdx.x] = kOctave[threadIdx.x];
+      const int group = tile_group(row.vectors), groups = ((row.vectors + 63) / 64 + group - 1) / group;
+      for (int i = threadIdx.x; i < kSums; i += kThreads) s.sums[i] = i < groups ? p.sums[(int64_t)r * kSums + i] : 0;
+      for (int i = 0, at = 0; i < p.slices; ++i) {
+        const int m = p.tops[(int64_t)r * p.slices + i].listed;
+        const uint64_t* from = p.lists + ((int64_t)r * p.slices + i) * kList;
+        for (int j = threadIdx.x; j < m; j += kThreads) s.list[at + j] = from[j];
+        at += m;
+      }
+      sort_list(s, n);
+      const Weight weight = octave_weight(temperature, octave, p.shift, s.table);
+      const uint64_t least = least_of(min_p, weight(split_z));
+      float cut_z = -INFINITY;
+      int cut_i = -1;
+      if (top_p < 1.f) {
+        const SplitRow x = p.split[r];
+        uint64_t c[2] = {0, 0}, w[2] = {0, 0}, sum, mine = 0;
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) row.first[k] = row.load(min(row.tile0 + k, row.tile1 - 1));
+        for (int e = 0; e < 2; ++e)
+          if (2 * (int)threadIdx.x + e < n) {
+            c[e] = s.list[2 * threadIdx.x + e];
+            w[e] = weight(candidate_z(c[e]));
+          }
+        const uint64_t b = x.ahead + block_before(w[0] + w[1], s, turn, &sum);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int i = 2 * threadIdx.x + e;
+          const bool in = i < n && (i == 0 || (double)(b + (e ? w[0] : 0)) < x.need);
+          mine += in ? 1 : 0;
+          if (in && w[e] >= least) {
+            const int tile = (candidate_at(c[e]) + row.lead) / (64 * E);
+            atomicAdd((unsigned long long*)&s.sums[tile / group], (unsigned long long)w[e]);
+          }
+        }
+        const uint64_t last = s.list[max((int)block_sum(mine, s, turn), 1) - 1];
+        cut_z = candidate_z(last);
+        cut_i = candidate_at(last);
+      }
+      __syncthreads();
+      pick_in_order<DT>(row, s, turn, group, [&](int tile, const float (&z)[E], auto add) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const uint64_t w = weight(z[j]);
+          const bool in = (z[j] > cut_z) | ((z[j] == cut_z) & (j <= cut_i - row.index(tile, 0)));
+          add(j, in & (w >= least) ? w : 0);
+        }
+      }, u, 0.0);
+      if (threadIdx.x == 0) answer(s.where, (float)((double)s.before / (double)s.total));
+      return;
+    }
   }
-  const bool greedy = !(temperature > 0.f);
-  const int k = top_k > 0 && top_k < p.V ? top_k : 0;
+  deal_tiles<DT>(row, 0, (row.vectors + 63) / 64);
   if (!greedy) {
     if (threadIdx.x < 64) s.table[threadIdx.x] = kOctave[threadIdx.x];
     if (k > 0)
@@ -411,10 +675,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
     row.inf = true;
     top = 0.f;
   }
-  const Weight weight{(double)top, 64.0 * 1.4426950408889634 / (double)temperature, p.shift, s.table};
+  const Weight weight{(double)top, kRate / (double)temperature, 0.0, p.shift, s.table};
   const uint64_t largest = 1ull << p.shift;
   // min-p: weights from `least` on stay (the largest always).
-  const uint64_t least = (uint64_t)fmin(fmax(ceil((double)min_p * (double)largest), 0.0), (double)largest);
+  const uint64_t least = least_of(min_p, largest);
   auto stays = [&](uint64_t w) { return w >= least; };
   // Kept: z > cut_z, or z == cut_z and i <= cut_i; without a cut, what is over -inf.
   float cut_z = -INFINITY;
@@ -699,23 +963,77 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
 
 }  // namespace
 
+namespace {
+
+// Workgroups that share a row: none where the rows fill the chip by themselves or a slice would be under 8192 logits
+// (64 rows of 128000, top-p: SPLIT1 us with one workgroup a row, SPLIT4 with four; one row of 50000: SPLITA, SPLITB).
+int slices_of(int rows, int V, int top_k_all, bool top_k_each) {
+  if (top_k_all > 0 && top_k_all < V && !top_k_each) return 0;
+  const int by_rows = axm_num_cus() / rows, by_size = V / 8192;
+  const int n = by_rows < by_size ? by_rows : by_size;
+  return n < 2 ? 0 : n < 16 ? n : 16;
+}
+struct SampleWorkspace {
+  size_t split, tops, sums, hists, lists, bytes;
+};
+SampleWorkspace sample_workspace(int rows, int slices) {
+  auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+  SampleWorkspace w{};
+  if (slices == 0) return w;
+  const size_t n = (size_t)rows * slices;
+  w.tops = w.split + up(rows * sizeof(SplitRow));
+  w.sums = w.tops + up(n * sizeof(SliceTop));
+  w.hists = w.sums + up((size_t)rows * kSums * 8);
+  w.lists = w.hists + up(n * kBins * 8);
+  w.bytes = w.lists + up(n * kList * 8);
+  return w;
+}
+
+template <int DT>
+void launch_sample(const SampleParams& p, int rows, hipStream_t s) {
+  if (p.slices > 0) {
+    hipLaunchKernelGGL((sample_slice_kernel<DT>), dim3(rows * p.slices), dim3(kThreads), 0, s, p);
+    hipLaunchKernelGGL((sample_sums_kernel<DT>), dim3(rows * p.slices), dim3(kThreads), 0, s, p);
+  }
+  hipLaunchKernelGGL((sample_kernel<DT>), dim3(rows), dim3(kThreads), 0, s, p);
+}
+
+}  // namespace
+
+extern "C" size_t axm_sample_rows_workspace_bytes(int rows, int V, int top_k_all, int top_k_each) {
+  if (rows < 1 || V < 1) return 0;
+  return sample_workspace(rows, slices_of(rows, V, top_k_all, top_k_each != 0)).bytes;
+}
+
 extern "C" int axm_sample_rows(const void* logits, int dtype, int64_t ld, int rows, int V, const float* u,
                                const float* temperature, const int* top_k, const float* top_p, const float* min_p,
                                float temperature_all, int top_k_all, float top_p_all, float min_p_all, int64_t* tokens,
-                               float* probs, void* stream) {
+                               float* probs, void* workspace, size_t workspace_bytes, void* stream) {
   AXM_CHECK_ARG(logits && u && tokens, -1, "sample_rows: null pointer");
   AXM_CHECK_ARG(dtype >= 0 && dtype <= 2, -1, "sample_rows: bad dtype %d", dtype);
   AXM_CHECK_ARG((uintptr_t)logits % (dtype == 1 ? 4 : 2) == 0, -1, "sample_rows: logits off their type's alignment");
   AXM_CHECK_ARG(rows >= 1 && rows < (1 << 22) && V >= 1 && V <= (1 << 24) && ld >= V, -1,
                 "sample_rows: %d rows of %d logits, %lld apart", rows, V, (long long)ld);
+  const int slices = slices_of(rows, V, top_k_all, top_k != nullptr);
+  const SampleWorkspace w = sample_workspace(rows, slices);
+  AXM_CHECK_ARG(workspace_bytes >= w.bytes && (w.bytes == 0 || (workspace && (uintptr_t)workspace % 16 == 0)), -1,
+                "sample_rows: workspace of %zu bytes needed (16-byte aligned), %zu given", w.bytes, workspace_bytes);
   int shift = 46;  // V 2^shift <= 2^63: no sum passes 64 bits
   while ((uint64_t)V << shift > 1ull << 63) --shift;
+  uint8_t* ws = (uint8_t*)workspace;
   SampleParams p{logits, ld, V, shift, u, temperature, top_k, top_p, min_p, temperature_all, top_p_all, min_p_all,
-                 top_k_all, tokens, probs};
+                 top_k_all, tokens, probs, slices, nullptr, nullptr, nullptr, nullptr, nullptr};
+  if (slices > 0) {
+    p.split = (SplitRow*)(ws + w.split);
+    p.tops = (SliceTop*)(ws + w.tops);
+    p.sums = (uint64_t*)(ws + w.sums);
+    p.hists = (uint64_t*)(ws + w.hists);
+    p.lists = (uint64_t*)(ws + w.lists);
+  }
   const hipStream_t s = (hipStream_t)stream;
-  if (dtype == 0) hipLaunchKernelGGL((sample_kernel<0>), dim3(rows), dim3(kThreads), 0, s, p);
-  else if (dtype == 1) hipLaunchKernelGGL((sample_kernel<1>), dim3(rows), dim3(kThreads), 0, s, p);
-  else hipLaunchKernelGGL((sample_kernel<2>), dim3(rows), dim3(kThreads), 0, s, p);
+  if (dtype == 0) launch_sample<0>(p, rows, s);
+  else if (dtype == 1) launch_sample<1>(p, rows, s);
+  else launch_sample<2>(p, rows, s);
   AXM_LAUNCH_CHECK("sample_rows");
   return 0;
 }

@@ -408,12 +408,17 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
         ld = z.stride(0) if rows > 1 else V
         if (V > 1 and z.stride(1) != 1) or ld < V:
             z, ld = z.contiguous(), V
+        k_all = min(k_all, V) if k is None else 0
         with on_device(dev.index):
-            rc = _lib.lib().axm_sample_rows(
+            L = _lib.lib()
+            need = L.axm_sample_rows_workspace_bytes(rows, V, k_all, 0 if k is None else 1)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            rc = L.axm_sample_rows(
                 z.data_ptr(), code, ld, rows, V, u.data_ptr(), None if t is None else t.data_ptr(),
                 None if k is None else k.data_ptr(), None if p is None else p.data_ptr(),
-                None if m is None else m.data_ptr(), t_all, min(k_all, V) if k is None else 0, p_all, m_all,
-                tokens.data_ptr(), None if probs is None else probs.data_ptr(), _lib.raw_stream(dev.index))
+                None if m is None else m.data_ptr(), t_all, k_all, p_all, m_all, tokens.data_ptr(),
+                None if probs is None else probs.data_ptr(), None if ws is None else ws.data_ptr(), need,
+                _lib.raw_stream(dev.index))
         if rc:
             _lib.check(rc, who)
     return (tokens, probs) if return_probs else tokens

@@ -59,6 +59,37 @@ def test_large_vocabularies(dev, dtype, V):
         check(z, u, *s)
 
 
+@pytest.mark.parametrize("dtype,V", [(torch.float16, 16384), (torch.float32, 20011), (torch.bfloat16, 65537),
+                                     (torch.float16, 131072), (torch.float32, 400003)])
+def test_few_rows_of_large_vocabularies_without_top_k(dev, dtype, V):
+    """Rows that several workgroups share: every slice with another largest logit, slices of -inf, ties over the slices'
+    borders, rows that are left to one workgroup (+inf, huge logits, temperatures near 0, too many ties at the cut)."""
+    inf = float("inf")
+    for rows, settings in ((1, SETTINGS), (9, SETTINGS[:1] + SETTINGS[3:4] + SETTINGS[6:7] + SETTINGS[10:])):
+        z, u = make_logits(dev, rows, V, dtype, V + rows)
+        for s in settings:
+            check(z, u, s[0], 0, s[2], s[3])
+    z, u = make_logits(dev, 12, V, dtype, V)
+    z[0] = z[0] + torch.linspace(-9, 9, V, device=dev).to(dtype)
+    z[1, : V // 2] = -inf
+    z[2, V // 3:] = -inf
+    z[3] = -inf
+    z[3, V - 1] = -7.0
+    z[4] = 0.25
+    z[5] = (torch.arange(V, device=dev) % 3).to(dtype)
+    z[6, V // 2] = inf
+    z[7] = z[7] * 3000
+    z[8] = z[8] * 0.001
+    z[9] = -inf
+    z[10] = z[10] - 300
+    z[11, ::7] = float("nan")
+    for s in [(1.0, 0.9, 0.0), (0.7, 1.0, 0.0), (1.3, 0.5, 0.02), (1e-3, 0.9, 0.0), (1e-7, 0.99, 0.0), (1e4, 0.3, 0.0),
+              (1.0, 0.0, 0.0), (1.0, 1.0, 0.3), (0.0, 0.9, 0.0)]:
+        check(z, u, s[0], 0, s[1], s[2])
+    k = torch.tensor([0, 5] * 6, device=dev, dtype=torch.int32)
+    check(z, u, torch.tensor([0.9, 0.0, 1.1] * 4, device=dev), k, torch.tensor([0.8, 1.0] * 6, device=dev), 0.01)
+
+
 def test_settings_of_every_row(dev):
     rows, V = 40, 5000
     z, u = make_logits(dev, rows, V, torch.float16, 3)

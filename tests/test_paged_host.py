@@ -81,7 +81,7 @@ def test_evict_refusals():
 
 def test_sampling_refusals():
     L = _lib.lib()
-    good = [P, 0, 100, 2, 100, P, None, None, None, None, 1.0, 0, 1.0, 0.0, P, None, None]
+    good = [P, 0, 100, 2, 100, P, None, None, None, None, 1.0, 0, 1.0, 0.0, P, None, None, 0, None]
     for at, value in ((0, None), (5, None), (14, None), (1, 3), (1, -1), (2, 99), (3, 0), (3, 1 << 22), (4, 0),
                       (4, (1 << 24) + 1)):
         args = list(good)
