@@ -19,7 +19,7 @@ constexpr int kBins = 2048;
 constexpr float kBinsPerUnit = 64.f;
 constexpr int kList = 2048;  // candidates in LDS
 constexpr int kAhead = 2;    // loads of a wave under way
-constexpr int kSums = 3072;  // entries of the running sum
+constexpr int kSums = 2048;  // entries of the running sum
 
 // 2^(j / 64), rounded to nearest.
 __device__ const double kOctave[64] = {
@@ -965,13 +965,15 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
 
 namespace {
 
-// Workgroups that share a row: none where the rows fill the chip by themselves or a slice would be under 8192 logits
-// (64 rows of 128000, top-p: SPLIT1 us with one workgroup a row, SPLIT4 with four; one row of 50000: SPLITA, SPLITB).
-int slices_of(int rows, int V, int top_k_all, bool top_k_each) {
-  if (top_k_all > 0 && top_k_all < V && !top_k_each) return 0;
-  const int by_rows = axm_num_cus() / rows, by_size = V / 8192;
-  const int n = by_rows < by_size ? by_rows : by_size;
-  return n < 2 ? 0 : n < 16 ? n : 16;
+// Workgroups that share a row, 8192 logits or more each: none where rows or vocabulary are too small for the three
+// launches to pay, or where top-k leaves rows a list that one workgroup is as fast with.  us, one workgroup a row / split:
+// with top-p 64 rows of 128000 93 / 51 (four slices), 100 of 50000 47 / 42 (two), 20 of 40000 36 / 32 (four), but 8 of
+// 30000 30 / 31 (three); without one row of 100000 42 / 21 (twelve), 60 of 50000 23 / 22 and in fp32 28 / 23 (four), but
+// 20 of 40000 19 / 21 (four) and 100 of 50000 23 / 26 (two); 60 of 20000 with top-k in most 26 / 45 (two).
+int slices_of(int rows, int V, bool top_k, bool top_p) {
+  const int by_rows = axm_num_cus() / rows, by_size = V / 8192, n = by_rows < by_size ? by_rows : by_size;
+  if (top_k || by_size < (top_p ? 4 : 5) || n < (top_p ? 2 : 4)) return 0;
+  return n < 16 ? n : 16;
 }
 struct SampleWorkspace {
   size_t split, tops, sums, hists, lists, bytes;
@@ -1000,9 +1002,9 @@ void launch_sample(const SampleParams& p, int rows, hipStream_t s) {
 
 }  // namespace
 
-extern "C" size_t axm_sample_rows_workspace_bytes(int rows, int V, int top_k_all, int top_k_each) {
+extern "C" size_t axm_sample_rows_workspace_bytes(int rows, int V, int with_top_k, int with_top_p) {
   if (rows < 1 || V < 1) return 0;
-  return sample_workspace(rows, slices_of(rows, V, top_k_all, top_k_each != 0)).bytes;
+  return sample_workspace(rows, slices_of(rows, V, with_top_k != 0, with_top_p != 0)).bytes;
 }
 
 extern "C" int axm_sample_rows(const void* logits, int dtype, int64_t ld, int rows, int V, const float* u,
@@ -1014,7 +1016,7 @@ extern "C" int axm_sample_rows(const void* logits, int dtype, int64_t ld, int ro
   AXM_CHECK_ARG((uintptr_t)logits % (dtype == 1 ? 4 : 2) == 0, -1, "sample_rows: logits off their type's alignment");
   AXM_CHECK_ARG(rows >= 1 && rows < (1 << 22) && V >= 1 && V <= (1 << 24) && ld >= V, -1,
                 "sample_rows: %d rows of %d logits, %lld apart", rows, V, (long long)ld);
-  const int slices = slices_of(rows, V, top_k_all, top_k != nullptr);
+  const int slices = slices_of(rows, V, top_k || (top_k_all > 0 && top_k_all < V), top_p || top_p_all < 1.f);
   const SampleWorkspace w = sample_workspace(rows, slices);
   AXM_CHECK_ARG(workspace_bytes >= w.bytes && (w.bytes == 0 || (workspace && (uintptr_t)workspace % 16 == 0)), -1,
                 "sample_rows: workspace of %zu bytes needed (16-byte aligned), %zu given", w.bytes, workspace_bytes);

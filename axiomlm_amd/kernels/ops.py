@@ -411,7 +411,7 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
         k_all = min(k_all, V) if k is None else 0
         with on_device(dev.index):
             L = _lib.lib()
-            need = L.axm_sample_rows_workspace_bytes(rows, V, k_all, 0 if k is None else 1)
+            need = L.axm_sample_rows_workspace_bytes(rows, V, k is not None or 0 < k_all < V, p is not None or p_all < 1.0)
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
             rc = L.axm_sample_rows(
                 z.data_ptr(), code, ld, rows, V, u.data_ptr(), None if t is None else t.data_ptr(),

@@ -325,10 +325,10 @@ int axm_evict_paged_kv(const axm_paged_kv* kv, int n_layer, int64_t layer_stride
  * with nothing to take gives -1 (and probability 0).  Settings: a device array of one per row, or NULL and the
  * value given.  probs fp32 [rows] or NULL: the token's share of the kept weights.  Sums are exact integers (weights are
  * rounded to 46 bits below the largest, fewer from 131072 logits on), so results do not depend on the order of threads.
- * workspace >= axm_sample_rows_workspace_bytes (0 for many rows, small vocabularies and a common top_k; top_k_each: whether
- * top_k is given per row).
+ * workspace >= axm_sample_rows_workspace_bytes (0 for many rows, small vocabularies and top-k; with_top_k, with_top_p: whether
+ * top_k is an array or in [1, V), top_p an array or under 1).
  * The reference samples in Python (axiomlm/engine/inference.py); next to axm_argmax. */
-size_t axm_sample_rows_workspace_bytes(int rows, int V, int top_k_all, int top_k_each);
+size_t axm_sample_rows_workspace_bytes(int rows, int V, int with_top_k, int with_top_p);
 int axm_sample_rows(const void* logits, int dtype, int64_t ld, int rows, int V, const float* u,
                     const float* temperature, const int* top_k, const float* top_p, const float* min_p,
                     float temperature_all, int top_k_all, float top_p_all, float min_p_all, int64_t* tokens,

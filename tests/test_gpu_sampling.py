@@ -59,7 +59,7 @@ def test_large_vocabularies(dev, dtype, V):
         check(z, u, *s)
 
 
-@pytest.mark.parametrize("dtype,V", [(torch.float16, 16384), (torch.float32, 20011), (torch.bfloat16, 65537),
+@pytest.mark.parametrize("dtype,V", [(torch.float16, 40960), (torch.float32, 50011), (torch.bfloat16, 65537),
                                      (torch.float16, 131072), (torch.float32, 400003)])
 def test_few_rows_of_large_vocabularies_without_top_k(dev, dtype, V):
     """Rows that several workgroups share: every slice with another largest logit, slices of -inf, ties over the slices'
@@ -86,8 +86,9 @@ def test_few_rows_of_large_vocabularies_without_top_k(dev, dtype, V):
     for s in [(1.0, 0.9, 0.0), (0.7, 1.0, 0.0), (1.3, 0.5, 0.02), (1e-3, 0.9, 0.0), (1e-7, 0.99, 0.0), (1e4, 0.3, 0.0),
               (1.0, 0.0, 0.0), (1.0, 1.0, 0.3), (0.0, 0.9, 0.0)]:
         check(z, u, s[0], 0, s[1], s[2])
-    k = torch.tensor([0, 5] * 6, device=dev, dtype=torch.int32)
-    check(z, u, torch.tensor([0.9, 0.0, 1.1] * 4, device=dev), k, torch.tensor([0.8, 1.0] * 6, device=dev), 0.01)
+    check(z, u, torch.tensor([0.9, 0.0, 1.1] * 4, device=dev), V, torch.tensor([0.8, 1.0] * 6, device=dev), 0.01)
+    check(z, u, torch.tensor([0.9, 0.0, 1.1] * 4, device=dev), torch.tensor([0, 5] * 6, device=dev),
+          torch.tensor([0.8, 1.0] * 6, device=dev), 0.01)
 
 
 def test_settings_of_every_row(dev):
