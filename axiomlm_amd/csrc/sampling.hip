@@ -20,26 +20,7 @@ constexpr float kBinsPerUnit = 64.f;
 constexpr int kList = 2048;  // candidates in LDS
 constexpr int kAhead = 2;    // loads of a wave under way
 constexpr int kSums = 2048;  // entries of the running sum
-
-// 2^(j / 64), rounded to nearest.
-__device__ const double kOctave[64] = {
-    1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
-    1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
-    1.0905077326652577, 1.1023825833078409, 1.1143867425958924, 1.1265216186082418,
-    1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812,
-    1.189207115002721, 1.2021567314527031, 1.215247359980469, 1.22848053610687,
-    1.241857812073484, 1.2553807570246911, 1.2690509571917332, 1.2828700160787783,
-    1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.3396675240533029,
-    1.3542555469368927, 1.3690024229745905, 1.383909881963832, 1.3989796725383112,
-    1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647,
-    1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384,
-    1.5422108254079407, 1.5590044002378369, 1.5759808451078865, 1.593142151342267,
-    1.6104903319492543, 1.6280274218573478, 1.6457554781539649, 1.6636765803267364,
-    1.681792830507429, 1.7001063537185235, 1.7186192981224779, 1.7373338352737062,
-    1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
-    1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
-    1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.9784560263879509,
-};
+constexpr int kTable = 512;  // entries of the table of 2^(j / kTable)
 
 struct SampleParams {
   const void* logits;
@@ -109,7 +90,7 @@ __device__ __forceinline__ uint64_t lane63(uint64_t x) {
 }
 
 struct Lds {
-  double table[64];  // of 2^(j / 64)
+  double table[kTable];  // of 2^(shift + j / kTable)
   union {
     struct {
       uint64_t weight[kBins];
@@ -271,31 +252,44 @@ struct Row {
   }
 };
 
-constexpr double kRate = 64.0 * 1.4426950408889634;
+constexpr double kRate = kTable * 1.4426950408889634;
 // Tiles of an entry of the running sum.
 __device__ __forceinline__ int tile_group(int vectors) { return ((vectors + 63) / 64 + kSums - 1) / kSums; }
 __device__ __forceinline__ int bin_of(float top, float z) {  // -inf and NaN: the last
   return (int)fminf((top - z) * kBinsPerUnit, (float)(kBins - 1));
 }
 
-// 2^shift 2^((z - top) rate / 64) as an integer: the table's 2^(j / 64) times a polynomial of the rest, at most
-// 2^-7 octaves either way (four terms: 2^-44 of the weight), rounded by adding 2^52.  z - top and what follows in 64
-// bits: differences of fp32 logits do not fit 32.
+// 2^shift 2^((z - top) rate / kTable) as an integer: the table's 2^(shift + j / kTable), with the whole octaves in its
+// exponent, times a polynomial of the rest, at most 2^-10 octaves either way (three terms: 2^-46 of the weight), rounded
+// by adding 2^52.  z - top and what follows in 64 bits: differences of fp32 logits do not fit 32.  128 octaves down and
+// beyond weigh 0.
 struct Weight {
-  double top, rate, off;  // rate: 64 log2(e) / T; off: added in 64ths of an octave
-  int shift;
+  double top, rate, off;  // rate: kTable log2(e) / T; off: added in kTable-ths of an octave
   const double* table;
   __device__ __forceinline__ uint64_t operator()(float z) const {
-    const double y = fmax(fma((double)z - top, rate, off), -64.0 * 1024.0);
+    const double y = fmax(fma((double)z - top, rate, off), -128.0 * kTable);
     const double near = y + 6755399441055744.0;  // 1.5 2^52: the nearest integer in the low bits
     const int i = (int)(uint32_t)__builtin_bit_cast(uint64_t, near);
     const double r = y - (near - 6755399441055744.0);
-    constexpr double a = 0.010830424696249145;  // ln 2 / 64
-    const double q = fma(fma(fma(fma(r, a * a * a * a / 24, a * a * a / 6), r, a * a / 2), r, a), r, 1.0);
-    const double w = ldexp(table[i & 63] * q, (i >> 6) + shift);
-    return __builtin_bit_cast(uint64_t, w + 4503599627370496.0) - 0x4330000000000000ull;
+    constexpr double a = 0.6931471805599453 / kTable;
+    const double q = fma(fma(fma(r, a * a * a / 6, a * a / 2), r, a), r, 1.0);
+    const uint64_t t = __builtin_bit_cast(uint64_t, table[i & (kTable - 1)]) + ((uint64_t)((uint32_t)(i & -kTable) * ((1u << 20) / kTable)) << 32);
+    return __builtin_bit_cast(uint64_t, fma(q, __builtin_bit_cast(double, t), 4503599627370496.0)) - 0x4330000000000000ull;
   }
 };
+__device__ __forceinline__ void fill_table(Lds& s, int shift) {
+  for (int j = threadIdx.x; j < kTable; j += kThreads) s.table[j] = ldexp(exp2((double)j / kTable), shift);
+}
+
+// Weights of a lane's logits, all of them before any is used: eight chains of 64-bit operations side by side.  Left to
+// itself the compiler moves each into the branch that uses it, one after the other.
+template <int E>
+__device__ __forceinline__ void weights_of(const Weight& weight, const float (&z)[E], uint64_t (&w)[E]) {
+#pragma unroll
+  for (int j = 0; j < E; ++j) w[j] = weight(z[j]);
+#pragma unroll
+  for (int j = 0; j < E; ++j) asm volatile("" : "+v"(w[j]));
+}
 
 // Sums of the weights of every `group` tiles, in s.sums; f(tile, z, add) calls add(j, weight) for the tile's logits that
 // have one.
@@ -430,33 +424,38 @@ __device__ __forceinline__ void deal_slice(Row<DT>& row, int slice, int slices) 
 }
 
 // ---------------------------------------------------------------------------
-// Few rows of large vocabularies, without top-k: `slices` workgroups a row.  First launch: every slice's largest logit and
-// its histogram of weights, over bins of a grid that all slices share (floor(64 z)) and relative to an octave of its
-// own; second: every slice adds the histograms up (shifted by whole bins and octaves), finds the bin with the cut, sums
-// its tiles' weights before that bin and lists the bin's candidates; third: one workgroup a row cuts the list, adds what
-// stays to the sums and picks the token.  Rows whose largest logit is infinite or passes 2^17 or 2^20 octaves,
-// and those that list too many, are left to the third launch, which then does everything.
+// Few rows of large vocabularies, without top-k: `slices` workgroups a row.  First launch: every slice's largest logit
+// and its histogram of weights, over bins of a grid that all slices share (64 z to the nearest integer) and relative to
+// an octave of its own; second: every slice adds the histograms up (shifted by whole bins and octaves), finds the bin
+// with the cut, sums its tiles' weights before that bin and lists the bin's candidates; third: one workgroup a row cuts
+// the list, adds what stays to the sums and picks the token.  Rows whose largest logit is infinite or passes 2^16 or 2^20
+// octaves, and those that list too many, are left to the third launch, which then does everything.  64 rows of 128000
+// with top-p: 15, 19 and 13 us, most of it the weights' 64-bit arithmetic (8 and 11 us; listing the kept logits first and
+// weighing those alone is slower: nuclei of thousands of tokens overflow the list).
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ float grid_of(float z) { return floorf(z * kBinsPerUnit); }
-__device__ __forceinline__ int grid_bin(float top_grid, float z) {
-  return (int)fminf(top_grid - grid_of(z), (float)(kBins - 1));
+__device__ __forceinline__ uint32_t grid_of(float z) {  // 1.5 2^23: the nearest integer in the low bits
+  return __builtin_bit_cast(uint32_t, fmaf(z, kBinsPerUnit, 12582912.f));
+}
+__device__ __forceinline__ int grid_bin(uint32_t top_grid, float z) {  // -inf and NaN: far past the last
+  return (int)min(top_grid - grid_of(z), (uint32_t)(kBins - 1));
 }
 // Weights of a split row: relative to whole octaves.
-__device__ __forceinline__ Weight octave_weight(float temperature, int octave, int shift, const double* table) {
-  return Weight{0.0, kRate / (double)temperature, -64.0 * (double)octave, shift, table};
+__device__ __forceinline__ Weight octave_weight(float temperature, int octave, const double* table) {
+  return Weight{0.0, kRate / (double)temperature, -(double)kTable * (double)octave, table};
 }
 // The row's largest logit and octave from its slices'; false: not to be split.
 __device__ __forceinline__ bool split_top(const SampleParams& p, int r, float* top, int* octave) {
-  float t = -INFINITY;
-  int o = -(1 << 30);
-  for (int i = 0; i < p.slices; ++i) {
-    const SliceTop x = p.tops[(int64_t)r * p.slices + i];
-    if (x.top > t) t = x.top;
-    o = max(o, x.octave);
+  const SliceTop x = p.tops[(int64_t)r * p.slices + min((int)threadIdx.x & 15, p.slices - 1)];  // (16 slices or fewer)
+  float t = x.top;
+  int o = x.octave;
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) {
+    t = fmaxf(t, __shfl_xor(t, d));
+    o = max(o, __shfl_xor(o, d));
   }
   *top = t;
   *octave = o;
-  return fabsf(t) < 131072.f && abs(o) < (1 << 20);  // (bins of larger logits are not whole in fp32)
+  return fabsf(t) < 65536.f && abs(o) < (1 << 20);  // (larger logits have coarser bins)
 }
 
 template <int DT>
@@ -469,7 +468,7 @@ __global__ void __launch_bounds__(kThreads) sample_slice_kernel(SampleParams p) 
   Row<DT> row = row_of<DT>(p, r);
   deal_slice<DT>(row, slice, p.slices);
   int turn = 0;
-  if (threadIdx.x < 64) s.table[threadIdx.x] = kOctave[threadIdx.x];
+  fill_table(s, p.shift);
   for (int i = threadIdx.x; i < kBins; i += kThreads) s.bins.weight[i] = 0;
   float top = -INFINITY;
   row.pass([&](int, const float (&z)[E]) {
@@ -478,19 +477,20 @@ __global__ void __launch_bounds__(kThreads) sample_slice_kernel(SampleParams p) 
   });
   const uint32_t best = (uint32_t)block_max(top > -INFINITY ? order_key(top) : 0, s, turn);
   top = best ? key_value(best) : -INFINITY;
-  const double octave = ceil((double)top * (kRate / 64.0) / (double)t.temperature);
+  const double octave = ceil((double)top * (kRate / kTable) / (double)t.temperature);
   const bool fine = best && fabs(octave) < (double)(1 << 20);
   if (threadIdx.x == 0)
     p.tops[blockIdx.x] = SliceTop{top, fine ? (int)octave : !best || octave < 0.0 ? -(1 << 30) : 1 << 30, 0};
   if (!fine || !(t.top_p < 1.f)) return;
-  const Weight weight = octave_weight(t.temperature, (int)octave, p.shift, s.table);
-  const float top_grid = grid_of(top);
+  const Weight weight = octave_weight(t.temperature, (int)octave, s.table);
+  const uint32_t top_grid = grid_of(top);
   row.pass([&](int, const float (&z)[E]) {
+    uint64_t w[E];
+    weights_of(weight, z, w);
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const uint64_t w = weight(z[j]);  // (of all: eight chains side by side)
-      if (z[j] > -INFINITY) atomicAdd((unsigned long long*)&s.bins.weight[grid_bin(top_grid, z[j])], (unsigned long long)w);
-    }
+    for (int j = 0; j < E; ++j)
+      if (z[j] > -INFINITY)
+        atomicAdd((unsigned long long*)&s.bins.weight[grid_bin(top_grid, z[j])], (unsigned long long)w[j]);
   });
   __syncthreads();
   uint64_t* to = p.hists + (int64_t)blockIdx.x * kBins;
@@ -514,24 +514,34 @@ __global__ void __launch_bounds__(kThreads) sample_sums_kernel(SampleParams p) {
   if (!split_top(p, r, &top, &octave)) return;
   Row<DT> row = row_of<DT>(p, r);
   deal_slice<DT>(row, slice, p.slices);
-  if (threadIdx.x < 64) s.table[threadIdx.x] = kOctave[threadIdx.x];
+  fill_table(s, p.shift);
   for (int i = threadIdx.x; i < kBins; i += kThreads) s.bins.weight[i] = 0;
   if (threadIdx.x == 0) s.n = 0, s.bin = 0, s.before = 0;
   __syncthreads();
-  const float top_grid = grid_of(top);
+  const uint32_t top_grid = grid_of(top);
   int bin = kBins;  // the bin with the cut; past the last: no top-p
   if (t.top_p < 1.f) {
-    for (int i = 0; i < p.slices; ++i) {
-      const SliceTop x = p.tops[(int64_t)r * p.slices + i];
-      const int down = octave - x.octave;
-      if (x.top == -INFINITY || down > 63) continue;
-      const int by = (int)fminf(top_grid - grid_of(x.top), (float)kBins);
-      const uint64_t* from = p.hists + ((int64_t)r * p.slices + i) * kBins;
+    constexpr int kTogether = 4;  // slices whose histograms are asked for together
+    for (int i0 = 0; i0 < p.slices; i0 += kTogether) {
+      uint64_t w[kTogether][kBins / kThreads];
+      SliceTop x[kTogether];
 #pragma unroll
-      for (int e = 0; e < kBins / kThreads; ++e) {
-        const int b = e * kThreads + threadIdx.x;
-        const uint64_t w = from[b] >> down;
-        if (w != 0) atomicAdd((unsigned long long*)&s.bins.weight[min(b + by, kBins - 1)], (unsigned long long)w);
+      for (int i = 0; i < kTogether; ++i) {
+        const int64_t n = (int64_t)r * p.slices + min(i0 + i, p.slices - 1);
+        x[i] = p.tops[n];
+#pragma unroll
+        for (int e = 0; e < kBins / kThreads; ++e) w[i][e] = p.hists[n * kBins + e * kThreads + threadIdx.x];
+      }
+#pragma unroll
+      for (int i = 0; i < kTogether; ++i) {
+        const int down = octave - x[i].octave;
+        if (i0 + i >= p.slices || x[i].top == -INFINITY || down > 63) continue;  // (the first: it has no histogram)
+        const int by = (int)min(top_grid - grid_of(x[i].top), (uint32_t)kBins);
+#pragma unroll
+        for (int e = 0; e < kBins / kThreads; ++e)
+          if (w[i][e] >> down != 0)
+            atomicAdd((unsigned long long*)&s.bins.weight[min(e * kThreads + (int)threadIdx.x + by, kBins - 1)],
+                      (unsigned long long)(w[i][e] >> down));
       }
     }
     __syncthreads();
@@ -548,16 +558,17 @@ __global__ void __launch_bounds__(kThreads) sample_sums_kernel(SampleParams p) {
     bin = s.bin;
     if (slice == 0 && threadIdx.x == 0) p.split[r] = SplitRow{need, s.before, bin};
   }
-  const Weight weight = octave_weight(t.temperature, octave, p.shift, s.table);
+  const Weight weight = octave_weight(t.temperature, octave, s.table);
   const uint64_t least = least_of(t.min_p, weight(top));
   uint64_t* list = p.lists + (int64_t)blockIdx.x * kList;
   const int group = tile_group(row.vectors);
   sum_tiles<DT>(row, s, group, [&](int tile, const float (&z)[E], auto add) {
+    uint64_t w[E];
+    weights_of(weight, z, w);
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-      const uint64_t w = weight(z[j]);
       const int b = grid_bin(top_grid, z[j]);
-      add(j, (z[j] > -INFINITY) & (b < bin) & (w >= least) ? w : 0);
+      add(j, (z[j] > -INFINITY) & (b < bin) & (w[j] >= least) ? w[j] : 0);
       if (b == bin && z[j] > -INFINITY) {
         const int at = atomicAdd(&s.n, 1);
         if (at < kList) list[at] = candidate(z[j], row.index(tile, j));
@@ -591,10 +602,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
   int octave;
   if (p.slices > 0 && !greedy && k == 0 && split_top(p, r, &split_z, &octave)) {
     // The slices have summed what lies before the bin with the cut and listed the bin.
-    int n = 0;
-    for (int i = 0; i < p.slices; ++i) n += p.tops[(int64_t)r * p.slices + i].listed;
+    int n = (threadIdx.x & 63) < p.slices ? p.tops[(int64_t)r * p.slices + (threadIdx.x & 63)].listed : 0;
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) n += __shfl_xor(n, d);
+    n = __builtin_amdgcn_readfirstlane(n);
     if (n <= kList) {
-      if (threadIdx.x < 64) s.table[threadIdx.x] = kOctave[threadIdx.x];
+      fill_table(s, p.shift);
       const int group = tile_group(row.vectors), groups = ((row.vectors + 63) / 64 + group - 1) / group;
       for (int i = threadIdx.x; i < kSums; i += kThreads) s.sums[i] = i < groups ? p.sums[(int64_t)r * kSums + i] : 0;
       for (int i = 0, at = 0; i < p.slices; ++i) {
@@ -604,7 +617,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
         at += m;
       }
       sort_list(s, n);
-      const Weight weight = octave_weight(temperature, octave, p.shift, s.table);
+      const Weight weight = octave_weight(temperature, octave, s.table);
       const uint64_t least = least_of(min_p, weight(split_z));
       float cut_z = -INFINITY;
       int cut_i = -1;
@@ -634,11 +647,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
       }
       __syncthreads();
       pick_in_order<DT>(row, s, turn, group, [&](int tile, const float (&z)[E], auto add) {
+        uint64_t w[E];
+        weights_of(weight, z, w);
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-          const uint64_t w = weight(z[j]);
           const bool in = (z[j] > cut_z) | ((z[j] == cut_z) & (j <= cut_i - row.index(tile, 0)));
-          add(j, in & (w >= least) ? w : 0);
+          add(j, in & (w[j] >= least) ? w[j] : 0);
         }
       }, u, 0.0);
       if (threadIdx.x == 0) answer(s.where, (float)((double)s.before / (double)s.total));
@@ -647,7 +661,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
   }
   deal_tiles<DT>(row, 0, (row.vectors + 63) / 64);
   if (!greedy) {
-    if (threadIdx.x < 64) s.table[threadIdx.x] = kOctave[threadIdx.x];
+    fill_table(s, p.shift);
     if (k > 0)
       for (int i = threadIdx.x; i < kBins; i += kThreads) s.bins.count[i] = 0;
     if (threadIdx.x == 0) s.n = 0, s.bin = -1;
@@ -675,7 +689,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
     row.inf = true;
     top = 0.f;
   }
-  const Weight weight{(double)top, kRate / (double)temperature, 0.0, p.shift, s.table};
+  const Weight weight{(double)top, kRate / (double)temperature, 0.0, s.table};
   const uint64_t largest = 1ull << p.shift;
   // min-p: weights from `least` on stay (the largest always).
   const uint64_t least = least_of(min_p, largest);
@@ -896,11 +910,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
     if (threadIdx.x == 0) s.n = 0, s.bin = 0, s.before = 0;
     __syncthreads();
     row.pass([&](int tile, const float (&z)[E]) {
+      uint64_t w[E];
+      weights_of(weight, z, w);
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const uint64_t w = weight(z[j]);  // (of all: eight chains side by side)
-        if (kept(z[j], tile, j)) atomicAdd((unsigned long long*)&s.bins.weight[bin_of(top, z[j])], (unsigned long long)w);
-      }
+      for (int j = 0; j < E; ++j)
+        if (kept(z[j], tile, j))
+          atomicAdd((unsigned long long*)&s.bins.weight[bin_of(top, z[j])], (unsigned long long)w[j]);
     });
     __syncthreads();
     uint64_t all;
@@ -952,11 +967,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
 #pragma unroll
     for (int j = 0; j < E; ++j) any |= z[j] >= cut_z;
     if (!__builtin_amdgcn_ballot_w64(any)) return;
+    uint64_t w[E];
+    weights_of(weight, z, w);
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const uint64_t w = weight(z[j]);
-      add(j, kept(z[j], tile, j) & stays(w) ? w : 0);
-    }
+    for (int j = 0; j < E; ++j) add(j, kept(z[j], tile, j) & stays(w[j]) ? w[j] : 0);
   }, u, 0.0);
   if (threadIdx.x == 0) answer(s.where, (float)((double)s.before / (double)s.total));
 }
