@@ -207,11 +207,14 @@ class PagedKVCache:
         self.k_scales = [None if self.scales is None else self.scales[i, 0] for i in range(n_layer)]
         self.v_scales = [None if self.scales is None else self.scales[i, 1] for i in range(n_layer)]
         self.block_table = torch.full((max_batch_size, self.max_pages), -1, dtype=torch.int32, device=device)
-        self.seq_lens = torch.zeros(max_batch_size, dtype=torch.int32, device=device)
+        # Rows: cached tokens; the same for sequences with a token in this step, 0 for the others.
+        self._lens = torch.zeros((2, max_batch_size), dtype=torch.int32, device=device)
+        self.seq_lens, self.step_lens = self._lens
         self.mass = torch.zeros((n_layer, max_batch_size, n_kv_head, self.max_seq_len), dtype=torch.float32,
                                 device=device) if account else None
         self.lens = [0] * max_batch_size       # cached tokens
         self.positions = [0] * max_batch_size  # tokens seen, evicted ones too: the next token's position
+        self._in_step = [False] * max_batch_size
         self._pages: list[list[int]] = [[] for _ in range(max_batch_size)]
         self._free = list(range(self.n_pages - 1, -1, -1))
 
@@ -226,7 +229,8 @@ class PagedKVCache:
         if table:
             rows = [p + [-1] * (self.max_pages - len(p)) for p in self._pages]
             self.block_table.copy_(torch.tensor(rows, dtype=torch.int32))
-        self.seq_lens.copy_(torch.tensor(self.lens, dtype=torch.int32))
+        step = [n if s else 0 for n, s in zip(self.lens, self._in_step)]
+        self._lens.copy_(torch.tensor([self.lens, step], dtype=torch.int32))
 
     def begin_step(self, counts: Sequence[int]) -> StepTokens:
         """Room for ``counts[b]`` new tokens of every sequence b (0: none); their sequences, positions and slots in
@@ -248,6 +252,7 @@ class PagedKVCache:
             slot += range(self.lens[b], self.lens[b] + c)
             self.positions[b] += c
             self.lens[b] += c
+        self._in_step = [c > 0 for c in counts]
         self._upload(sum(need) > 0)
         dev = self.cache.device
         return StepTokens(*torch.tensor([seq, pos, slot], dtype=torch.int32).to(dev))
@@ -262,9 +267,9 @@ class PagedKVCache:
                                   kv_dtype=self.cache_dtype)
 
     def attend(self, layer: int, q: torch.Tensor) -> torch.Tensor:
-        """Attention of q (B, Hq, hd), one token per sequence, over all that the layer holds; with ``account`` its
-        weights join ``mass``.  Sequences without a token give zeros."""
-        return gqa_paged_decode(q, self.k_caches[layer], self.v_caches[layer], self.block_table, self.seq_lens,
+        """Attention of q (B, Hq, hd), the step's last token of every sequence, over all that the layer holds of it; with
+        ``account`` its weights join ``mass``.  Sequences without a token in this step give zeros."""
+        return gqa_paged_decode(q, self.k_caches[layer], self.v_caches[layer], self.block_table, self.step_lens,
                                 self.k_scales[layer], self.v_scales[layer], self.cache_dtype,
                                 None if self.mass is None else self.mass[layer])
 
@@ -291,6 +296,7 @@ class PagedKVCache:
         """End sequence ``seq``: its pages go back to the pool."""
         self._keep(seq, 0)
         self.positions[seq] = 0
+        self._in_step[seq] = False
         if self.mass is not None:
             self.mass[:, seq].zero_()
         self._upload(True)
@@ -299,6 +305,7 @@ class PagedKVCache:
         for b in range(self.max_batch_size):
             self._keep(b, 0)
             self.positions[b] = 0
+            self._in_step[b] = False
         if self.mass is not None:
             self.mass.zero_()
         self._upload(True)

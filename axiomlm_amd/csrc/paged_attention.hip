@@ -629,8 +629,10 @@ void launch_decode(const DecodeParams& p, hipStream_t s) {
   else launch_decode_rows<KVT, HD, false>(p, s);
 }
 
-// Up to this many blocks of capacity a workgroup takes a pair whole and nothing is joined by a second launch.
-constexpr int kPairBlocks = 16;
+// Up to this many blocks of capacity a workgroup takes a pair whole and nothing is joined by a second launch (us, one
+// launch / two; fp16, 8 KV heads of 128: one sequence of 100 keys 5.4 / 7.2, of 256 8.9 / 10.0, 16 of 250 8.9 / 10.4; one of
+// 500 12.1 / 10.2, 64 of 500 19.2 / 17.9, one of 1000 19.0 / 10.1).
+constexpr int kPairBlocks = 8;
 
 // Workgroups of the first launch otherwise; no more than have a block at the table's capacity.  Per CU two where rows
 // are long, three where a wave's registers and its steps' bytes are few (128 sequences, INT4, heads of 64: 28.4 us with
@@ -717,7 +719,8 @@ extern "C" int axm_paged_flash_decode(const void* q, int64_t ld_q, const axm_pag
     default: launch_decode<AXM_KV_INT4, 128>(p, s); break;
   }
   AXM_LAUNCH_CHECK("paged_flash_decode");
-  // One wave a row where a pair has few parts (about grid / pairs, one more), four where it has many.
+  // One wave a row where a pair has few parts (about grid / pairs, one more), four where it has many (us, one / four: 128
+  // INT4 sequences 25.2 / 27.9, 48 fp16 ones 49.8 / 50.3; 8 INT4 ones of 4000 keys 15.4 / 11.7, one FP8 one of 8000 23.2 / 15.3).
   const bool many = parts && (int64_t)p.grid > 4 * (int64_t)kv.n_seqs * kv.Hkv * p.chunks;
   const int rows = kv.n_seqs * n_head, join = !parts ? 0 : many ? rows : (rows + kWaves - 1) / kWaves;
   const int account = mass ? kv.n_seqs * kv.Hkv * slices : 0;

@@ -363,10 +363,12 @@ def _setting(who: str, name: str, x, dtype: torch.dtype, rows: int, device, low:
             if x.device != device or x.numel() != rows:
                 raise ValueError(f"{who}: {name} must have one entry per row ({rows}) on {device}, got "
                                  f"{tuple(x.shape)} on {x.device}")
+            if x.dtype == torch.int64 and dtype == torch.int32:
+                x = x.clamp(-2**31, 2**31 - 1)
             return x.to(dtype).contiguous(), 0
         x = x.item()
-    if not low <= x <= high:
-        raise ValueError(f"{who}: {name}={x} outside [{low}, {high}]")
+    if not low <= x <= high or (dtype == torch.int32 and x != _INF and x != int(x)):
+        raise ValueError(f"{who}: {name}={x} outside [{low}, {high}]" + (" or not whole" if low <= x <= high else ""))
     return None, x
 
 
@@ -408,7 +410,7 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0,
         ld = z.stride(0) if rows > 1 else V
         if (V > 1 and z.stride(1) != 1) or ld < V:
             z, ld = z.contiguous(), V
-        k_all = min(k_all, V) if k is None else 0
+        k_all = int(min(k_all, V)) if k is None else 0
         with on_device(dev.index):
             L = _lib.lib()
             need = L.axm_sample_rows_workspace_bytes(rows, V, k is not None or 0 < k_all < V, p is not None or p_all < 1.0)

@@ -26,12 +26,14 @@ _PAGED_KV = struct.Struct("5P2q7i4x")  # axm_paged_kv (include/axm.h)
 
 
 def _ints(who: str, name: str, t: torch.Tensor, device: torch.device, n: int) -> torch.Tensor:
-    """A device array of n int32 (int64 is converted)."""
+    """A device array of n int32 (int64 is converted; what does not fit stays out of range)."""
     if not isinstance(t, torch.Tensor) or t.device != device or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{who}: {name} must be an int32 or int64 tensor on {device}")
     if t.dim() != 1 or t.numel() != n:
         raise ValueError(f"{who}: {name} has shape {tuple(t.shape)}, expected ({n},)")
-    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+    if t.dtype == torch.int64:
+        t = t.clamp(-2**31, 2**31 - 1).to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _page_stride(who: str, name: str, t: torch.Tensor) -> int:

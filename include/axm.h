@@ -296,7 +296,7 @@ int axm_rope_paged_kv_write(void* qkv, int64_t ld_qkv, int T, const void* freqs,
  * page_size]); keys and values as axm_dequantize_kv gives them.  A sequence of length 0 gives zeros; keys on a page
  * outside the pool are left out.  mass (or NULL): fp32 [n_seqs][Hkv][mass_len], mass_len >= max_pages page_size;
  * the softmax weights of slot s, summed over the query heads of the KV head, are added to mass[b][kvh][s].
- * workspace >= axm_paged_decode_workspace_bytes (256-byte aligned). */
+ * out and workspace (>= axm_paged_decode_workspace_bytes) are 16-byte aligned. */
 size_t axm_paged_decode_workspace_bytes(int n_seqs, int n_head, int n_kv_head, int head_dim, int page_size,
                                         int max_pages, int with_mass);
 int axm_paged_flash_decode(const void* q, int64_t ld_q, const axm_paged_kv* kv, const int* seq_lens, void* out,
@@ -310,7 +310,7 @@ int axm_paged_flash_decode(const void* q, int64_t ld_q, const axm_paged_kv* kv, 
  * rows behind stay as they are).  mass fp32 [L][n_seqs][Hkv][mass_len] is read; mass_out (same shape, another buffer) has
  * the kept slots' values and zeros behind them; kept int32 [L][n_seqs][Hkv][budget] the slots that the rows come from
  * (-1 behind the last); lens_out int32 [n_seqs] = min(seq_lens, budget).  1 <= budget, 0 <= recent <= budget.  Pages
- * of a sequence over the budget must not be shared with another one. */
+ * of a sequence over the budget must not be shared with another one, nor k's with v. */
 int axm_evict_paged_kv(const axm_paged_kv* kv, int n_layer, int64_t layer_stride, int64_t scale_layer_stride,
                        const int* seq_lens, const float* mass, int64_t mass_len, int budget, int recent,
                        float* mass_out, int* kept, int* lens_out, void* stream);
@@ -325,8 +325,8 @@ int axm_evict_paged_kv(const axm_paged_kv* kv, int n_layer, int64_t layer_stride
  * with nothing to take gives -1 (and probability 0).  Settings: a device array of one per row, or NULL and the
  * value given.  probs fp32 [rows] or NULL: the token's share of the kept weights.  Sums are exact integers (weights are
  * rounded to 46 bits below the largest, fewer from 131072 logits on), so results do not depend on the order of threads.
- * workspace >= axm_sample_rows_workspace_bytes (0 for many rows, small vocabularies and top-k; with_top_k, with_top_p: whether
- * top_k is an array or in [1, V), top_p an array or under 1).
+ * workspace >= axm_sample_rows_workspace_bytes, 16-byte aligned (0 for many rows, small vocabularies and top-k;
+ * with_top_k, with_top_p: whether top_k is an array or in [1, V), top_p an array or under 1).
  * The reference samples in Python (axiomlm/engine/inference.py); next to axm_argmax. */
 size_t axm_sample_rows_workspace_bytes(int rows, int V, int with_top_k, int with_top_p);
 int axm_sample_rows(const void* logits, int dtype, int64_t ld, int rows, int V, const float* u,

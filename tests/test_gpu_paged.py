@@ -175,6 +175,8 @@ def test_lengths_past_the_table_are_held_to_it(dev):
     want = K.gqa_paged_decode(q[:1], k, v, table[:1], n[:1])
     got = K.gqa_paged_decode(q, k, v, table, torch.tensor([10**9, -5], dtype=torch.int32, device=dev))
     assert torch.equal(got[0], want[0]) and bool((got[1] == 0).all())
+    got = K.gqa_paged_decode(q, k, v, table, torch.tensor([2**32 + 5, -2**32 + 5], device=dev))
+    assert torch.equal(got[0], want[0]) and bool((got[1] == 0).all())
 
 
 def test_shared_pages_and_repeated_rows(dev):
@@ -467,6 +469,11 @@ def test_write_rows_may_be_strided_and_int64(dev):
     for t in range(2):
         s = int(pos[t])
         assert torch.equal(v[int(table[t, s // 16]), :, s % 16], rows[t, (H + Hkv) * hd:(H + 2 * Hkv) * hd].view(Hkv, hd))
+    # Slots and sequences that 32 bits would bring back into range are padding.
+    was, row = pool.clone(), wide.clone()
+    K.rope_paged_kv_cache_write(qkv, fr, k, v, table, pos, H * hd, Hkv * hd, hd, slots=torch.tensor([2**32, 5], device=dev),
+                                seq_ids=torch.tensor([0, 2**32 + 1], device=dev))
+    assert torch.equal(pool, was) and torch.equal(wide, row)
 
 
 def test_write_refusals(dev):

@@ -116,6 +116,13 @@ def test_ties(dev, dtype):
             check(z, u, *s)
 
 
+def test_top_k_past_32_bits_is_no_filter(dev):
+    z, u = make_logits(dev, 3, 500, torch.float16, 12)
+    want = K.sample_tokens(z, u)
+    assert torch.equal(K.sample_tokens(z, u, top_k=2**32 + 1), want)
+    assert torch.equal(K.sample_tokens(z, u, top_k=torch.tensor([2**32 + 1, 2**31, -2**32 + 1], device=dev)), want)
+
+
 def test_signed_zeros_are_equal(dev):
     z = torch.full((1, 100), -0.0, device=dev)
     z[0, 50:] = 0.0
@@ -223,6 +230,6 @@ def test_refusals(dev):
     z, u = make_logits(dev, 2, 100, torch.float16, 11)
     for args in ((z.double(), u), (z.long(), u), (z, u[:1]), (z, u.double()), (z, u.cpu()), (z[:, :0], u), (z.cpu(), u),
                  (z, u, -1.0), (z, u, float("nan")), (z, u, 1.0, -1), (z, u, 1.0, 0, 1.5), (z, u, 1.0, 0, -0.1),
-                 (z, u, 1.0, 0, 1.0, 1.1), (z, u, torch.ones(3, device=dev)), (z, u, torch.ones(2))):
+                 (z, u, 1.0, 5.5), (z, u, 1.0, 0, 1.0, 1.1), (z, u, torch.ones(3, device=dev)), (z, u, torch.ones(2))):
         with pytest.raises((ValueError, RuntimeError)):
             K.sample_tokens(*args)

@@ -14,7 +14,7 @@ P = 4096  # an address that is never followed
 
 
 def desc(**change):
-    d = dict(k=P, v=P, k_scales=P, v_scales=P, block_table=P, page_stride=2 * 16 * 128, scale_stride=2 * 16 * 2,
+    d = dict(k=P, v=2 * P, k_scales=P, v_scales=P, block_table=P, page_stride=2 * 16 * 128, scale_stride=2 * 16 * 2,
              kv_dtype=0, n_kv_head=2, head_dim=64, page_size=16, n_pages=3, n_seqs=2, max_pages=4)
     d.update(change)
     return _lib.PagedKv(**d)
@@ -77,6 +77,7 @@ def test_evict_refusals():
         args = list(good)
         args[at] = value
         refused(L.axm_evict_paged_kv(*args))
+    refused(L.axm_evict_paged_kv(ctypes.byref(desc(v=P)), *good[1:]), "same pages")
 
 
 def test_sampling_refusals():
