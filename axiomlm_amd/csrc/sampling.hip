@@ -35,6 +35,7 @@ struct SampleParams {
   int top_k_all;
   int64_t* tokens;
   float* probs;
+  bool order;  // rows with top-p and no top-k first
   // Few rows: `slices` workgroups share a row without top-k (SplitRow); 0: none do.
   int slices;
   struct SliceTop* tops;  // [rows][slices]
@@ -392,6 +393,21 @@ __device__ __forceinline__ Settings settings_of(const SampleParams& p, int r) {
   return t;
 }
 
+// The row of this workgroup where those with top-p and no top-k, which take longest, start first: where more rows than
+// fit the chip at once have settings of their own, some of them would run alone at the end.  us, as they come / slow ones
+// first: 500 rows of 50304 in fp32 95.5 / 86.3, 300 in fp16 57.7 / 50.7, 1000 rows of 128000 247 / 205; but 1000 of 32000
+// 98 / 102 and 400 of 20000 47 / 50 (finding the row takes 2 us of each), so large vocabularies only.
+__device__ __forceinline__ int row_in_order(const SampleParams& p, Lds& s, int& turn) {
+  const int rows = gridDim.x, mine = threadIdx.x, wanted = blockIdx.x;
+  const Settings t = settings_of(p, min(mine, rows - 1));
+  const bool slow = mine < rows && !t.greedy && t.k == 0 && t.top_p < 1.f;
+  uint64_t total;
+  const int before = (int)block_before(slow, s, turn, &total);
+  if (mine < rows && (slow ? before : (int)total + mine - before) == wanted) s.where = mine;
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(s.where);
+}
+
 // Row r, with the tiles [tile0, tile1) of a workgroup dealt to its waves in contiguous runs.
 template <int DT>
 __device__ __forceinline__ Row<DT> row_of(const SampleParams& p, int r) {
@@ -585,7 +601,9 @@ template <int DT>
 __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
   constexpr int E = Row<DT>::E;
   __shared__ Lds s;
-  const int r = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int turn = 0;
+  const int r = p.order ? row_in_order(p, s, turn) : blockIdx.x;
   Row<DT> row = row_of<DT>(p, r);
   const Settings settings = settings_of(p, r);
   const float temperature = settings.temperature, top_p = settings.top_p, min_p = settings.min_p;
@@ -593,7 +611,6 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
   const int k = settings.k;
   const double u = fmin(fmax((double)p.u[r], 0.0), 1.0);  // (NaN: 0)
 
-  int turn = 0;
   auto answer = [&](int token, float prob) {
     p.tokens[r] = token;
     if (p.probs) p.probs[r] = prob;
@@ -1038,7 +1055,9 @@ extern "C" int axm_sample_rows(const void* logits, int dtype, int64_t ld, int ro
   while ((uint64_t)V << shift > 1ull << 63) --shift;
   uint8_t* ws = (uint8_t*)workspace;
   SampleParams p{logits, ld, V, shift, u, temperature, top_k, top_p, min_p, temperature_all, top_p_all, min_p_all,
-                 top_k_all, tokens, probs, slices, nullptr, nullptr, nullptr, nullptr, nullptr};
+                 top_k_all, tokens, probs,
+                 V >= 40960 && rows > axm_num_cus() && rows <= kThreads && (temperature || top_k || top_p),
+                 slices, nullptr, nullptr, nullptr, nullptr, nullptr};
   if (slices > 0) {
     p.split = (SplitRow*)(ws + w.split);
     p.tops = (SliceTop*)(ws + w.tops);

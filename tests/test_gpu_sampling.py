@@ -103,6 +103,16 @@ def test_settings_of_every_row(dev):
     check(z, u, t.double(), k.long(), 0.9, r() * 0.1)
 
 
+def test_more_rows_than_fit_at_once_with_settings_of_their_own(dev):
+    rows, V = 300, 41001
+    z, u = make_logits(dev, rows, V, torch.float16, 13)
+    i = torch.arange(rows, device=dev)
+    z[7], z[299] = float("-inf"), float("-inf")
+    z[11, 5] = float("inf")
+    check(z, u, torch.where(i % 5 == 0, 0.0, 0.6 + (i % 7) / 8.0), (i % 3) * 40, torch.where(i % 4 == 1, 1.0, 0.85), 0.01)
+    check(z[:257], u[:257], 0.9, 0, torch.where(i[:257] % 2 == 0, 1.0, 0.7), 0.0)
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 def test_ties(dev, dtype):
     """Equal logits at the borders: the lower index is kept."""
