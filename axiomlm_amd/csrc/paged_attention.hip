@@ -129,9 +129,11 @@ struct Piece {
 };
 
 // NV: query rows of a lane (4 NV or fewer rows in all).  Row r is tile row 4 (r % 4) + r / 4, so that the lanes of a tile
-// share the rows evenly: with four heads per KV head every lane has one row to weigh instead of some lanes four.
-// SPLIT: pages of 16 tokens, so the two halves of a block lie on pages of their own.
-template <int KVT, int HD, int NV, bool SPLIT>
+// share the rows evenly: with four heads per KV head every lane has one row to weigh instead of some lanes four (us, NV by
+// the rows / always 4: 128 INT4 sequences of 8 rows 25.5 / 28.0, one sequence of one row 5.4 / 6.0, 48 fp16 ones 50.7 / 51.0).
+// Each half of a block has its page looked up: it may be another one with pages of 16, and one lookup for both where it
+// is not was no faster (48 fp16 sequences, pages of 64: 50.7 with one, 49.8 with two).
+template <int KVT, int HD, int NV>
 __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(DecodeParams p) {
   using S = RowShape<KVT, HD>;
   constexpr int KS = HD / 32, DT = HD / 16;
@@ -211,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(DecodeParams 
       }
       const const_ints table = as_const(kv.table) + (int64_t)x.b * kv.max_pages;
       x.page[0] = table[x.c * kBlock >> kv.page_shift];
-      x.page[1] = SPLIT ? table[min(x.c * kBlock + 16, x.len - 1) >> kv.page_shift] : x.page[0];
+      x.page[1] = table[min(x.c * kBlock + 16, x.len - 1) >> kv.page_shift];
       if (--left > 0 && ++lead.c == lead.n) {
         lead.c = 0;
         if (++lead.chunk == p.chunks) {
@@ -232,14 +234,13 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(DecodeParams 
     };
     // Rows past the sequence, and those of a page outside the pool, are past their descriptors' ends and read as zeros.
     auto fetch = [&](const Block& x, Step<KVT, HD>& st) {
-      constexpr int kHalf = SPLIT ? 16 : 32;  // keys of a descriptor
       const int mask = (1 << kv.page_shift) - 1;
 #pragma unroll
-      for (int part = 0; part < kBlock / kHalf; ++part) {
-        const bool ok = (unsigned)x.page[part] < (unsigned)kv.n_pages;
-        const int n = ok ? min(max(x.len - x.c * kBlock - 16 * part, 0), kHalf) : 0;
-        const int64_t page = ok ? x.page[part] : 0;
-        const int row = (x.kvh << kv.page_shift) + ((x.c * kBlock + 16 * part) & mask);
+      for (int h = 0; h < 2; ++h) {
+        const bool ok = (unsigned)x.page[h] < (unsigned)kv.n_pages;
+        const int n = ok ? min(max(x.len - x.c * kBlock - 16 * h, 0), 16) : 0;
+        const int64_t page = ok ? x.page[h] : 0;
+        const int row = (x.kvh << kv.page_shift) + ((x.c * kBlock + 16 * h) & mask);
         const int64_t off = page * kv.page_stride + row * S::kBytes;
         const auto kr = rows_at(kv.k, off, n * S::kBytes);
         const auto vr = rows_at(kv.v, off, n * S::kBytes);
@@ -249,31 +250,27 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(DecodeParams 
           ksr = rows_at(kv.ks, so, n * S::kScale);
           vsr = rows_at(kv.vs, so, n * S::kScale);
         }
+        const int lo = l16 * S::kBytes + lq * S::kLoad;
 #pragma unroll
-        for (int h = part; h < part + kHalf / 16; ++h) {
-          const int lo = (l16 + (SPLIT ? 0 : 16 * h)) * S::kBytes + lq * S::kLoad;
-#pragma unroll
-          for (int j = 0; j < S::kLoads; ++j) {
-            if constexpr (S::kLoad == 16) {
-              st.k[h][j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kr, lo + 64 * j, 0, 0));
-              st.v[h][j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vr, lo + 64 * j, 0, 0));
-            } else {
-              const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(kr, lo, 0, 0));
-              const u32x2 d = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(vr, lo, 0, 0));
-              st.k[h][j] = u32x4{a.x, a.y, 0u, 0u};
-              st.v[h][j] = u32x4{d.x, d.y, 0u, 0u};
-            }
+        for (int j = 0; j < S::kLoads; ++j) {
+          if constexpr (S::kLoad == 16) {
+            st.k[h][j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kr, lo + 64 * j, 0, 0));
+            st.v[h][j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vr, lo + 64 * j, 0, 0));
+          } else {
+            const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(kr, lo, 0, 0));
+            const u32x2 d = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(vr, lo, 0, 0));
+            st.k[h][j] = u32x4{a.x, a.y, 0u, 0u};
+            st.v[h][j] = u32x4{d.x, d.y, 0u, 0u};
           }
-          st.ks[h] = st.vs[h] = 0u;
-          if constexpr (KVT != AXM_KV_FP16) {
-            const int slo = (l16 + (SPLIT ? 0 : 16 * h)) * S::kScale;
-            if constexpr (HD == 128) {
-              st.ks[h] = __builtin_amdgcn_raw_buffer_load_b32(ksr, slo, 0, 0);
-              st.vs[h] = __builtin_amdgcn_raw_buffer_load_b32(vsr, slo, 0, 0);
-            } else {
-              st.ks[h] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(ksr, slo, 0, 0);
-              st.vs[h] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(vsr, slo, 0, 0);
-            }
+        }
+        st.ks[h] = st.vs[h] = 0u;
+        if constexpr (KVT != AXM_KV_FP16) {
+          if constexpr (HD == 128) {
+            st.ks[h] = __builtin_amdgcn_raw_buffer_load_b32(ksr, l16 * S::kScale, 0, 0);
+            st.vs[h] = __builtin_amdgcn_raw_buffer_load_b32(vsr, l16 * S::kScale, 0, 0);
+          } else {
+            st.ks[h] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(ksr, l16 * S::kScale, 0, 0);
+            st.vs[h] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(vsr, l16 * S::kScale, 0, 0);
           }
         }
       }
@@ -614,19 +611,14 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(DecodeParams p, in
   }
 }
 
-template <int KVT, int HD, bool SPLIT>
-void launch_decode_rows(const DecodeParams& p, hipStream_t s) {
+template <int KVT, int HD>
+void launch_decode(const DecodeParams& p, hipStream_t s) {
   const int rows = p.n_rep < kRows ? p.n_rep : kRows;
   const size_t lds = kWaves * ((kBlock * (HD + 16) + 2 * kRows * kBlock) * 2 + rows * (2 + HD) * 4);
   const dim3 grid(p.grid), block(kThreads);
-  if (rows <= 4) hipLaunchKernelGGL((paged_decode_kernel<KVT, HD, 1, SPLIT>), grid, block, lds, s, p);
-  else if (rows <= 8) hipLaunchKernelGGL((paged_decode_kernel<KVT, HD, 2, SPLIT>), grid, block, lds, s, p);
-  else hipLaunchKernelGGL((paged_decode_kernel<KVT, HD, 4, SPLIT>), grid, block, lds, s, p);
-}
-template <int KVT, int HD>
-void launch_decode(const DecodeParams& p, hipStream_t s) {
-  if (p.kv.page_shift == 4) launch_decode_rows<KVT, HD, true>(p, s);
-  else launch_decode_rows<KVT, HD, false>(p, s);
+  if (rows <= 4) hipLaunchKernelGGL((paged_decode_kernel<KVT, HD, 1>), grid, block, lds, s, p);
+  else if (rows <= 8) hipLaunchKernelGGL((paged_decode_kernel<KVT, HD, 2>), grid, block, lds, s, p);
+  else hipLaunchKernelGGL((paged_decode_kernel<KVT, HD, 4>), grid, block, lds, s, p);
 }
 
 // Up to this many blocks of capacity a workgroup takes a pair whole and nothing is joined by a second launch (us, one

@@ -101,7 +101,7 @@ struct Lds {
   };
   uint64_t list[kList];
   uint64_t red[2][kWaves];
-  uint64_t total, before, cut;
+  uint64_t total, before;
   int n, bin, where;
   int small[64];
 };
