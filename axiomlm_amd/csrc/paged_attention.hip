@@ -129,8 +129,9 @@ struct Piece {
 };
 
 // NV: query rows of a lane (4 NV or fewer rows in all).  Row r is tile row 4 (r % 4) + r / 4, so that the lanes of a tile
-// share the rows evenly: with four heads per KV head every lane has one row to weigh instead of some lanes four (us, NV by
-// the rows / always 4: 128 INT4 sequences of 8 rows 25.5 / 28.0, one sequence of one row 5.4 / 6.0, 48 fp16 ones 50.7 / 51.0).
+// share the rows evenly: with four heads per KV head every lane has one row to weigh instead of some lanes four (us, NV
+// by the rows / always 4: 128 INT4 sequences of 8 rows 25.5 / 28.0, one sequence of one row 5.4 / 6.0, 48 fp16 ones of
+// four 50.7 / 51.0).
 // Each half of a block has its page looked up: it may be another one with pages of 16, and one lookup for both where it
 // is not was no faster (48 fp16 sequences, pages of 64: 50.7 with one, 49.8 with two).
 template <int KVT, int HD, int NV>
@@ -622,8 +623,8 @@ void launch_decode(const DecodeParams& p, hipStream_t s) {
 }
 
 // Up to this many blocks of capacity a workgroup takes a pair whole and nothing is joined by a second launch (us, one
-// launch / two; fp16, 8 KV heads of 128: one sequence of 100 keys 5.4 / 7.2, of 256 8.9 / 10.0, 16 of 250 8.9 / 10.4; one of
-// 500 12.1 / 10.2, 64 of 500 19.2 / 17.9, one of 1000 19.0 / 10.1).
+// launch / two; fp16: one sequence of 100 keys, 4 heads of 64, 5.4 / 7.2; 8 KV heads of 128: one of 256 8.9 / 10.0, 16 of
+// 250 8.9 / 10.4; one of 500 12.1 / 10.2, 64 of 500 19.2 / 17.9, one of 1000 19.0 / 10.1).
 constexpr int kPairBlocks = 8;
 
 // Workgroups of the first launch otherwise; no more than have a block at the table's capacity.  Per CU two where rows
@@ -711,8 +712,9 @@ extern "C" int axm_paged_flash_decode(const void* q, int64_t ld_q, const axm_pag
     default: launch_decode<AXM_KV_INT4, 128>(p, s); break;
   }
   AXM_LAUNCH_CHECK("paged_flash_decode");
-  // One wave a row where a pair has few parts (about grid / pairs, one more), four where it has many (us, one / four: 128
-  // INT4 sequences 25.2 / 27.9, 48 fp16 ones 49.8 / 50.3; 8 INT4 ones of 4000 keys 15.4 / 11.7, one FP8 one of 8000 23.2 / 15.3).
+  // One wave a row where a pair has few parts (about grid / pairs, one more), four where it has many (us, one / four:
+  // 128 INT4 sequences 25.2 / 27.9, 48 fp16 ones 49.8 / 50.3; 8 INT4 ones of 4000 keys 15.4 / 11.7, one FP8 one of 8000
+  // 23.2 / 15.3).
   const bool many = parts && (int64_t)p.grid > 4 * (int64_t)kv.n_seqs * kv.Hkv * p.chunks;
   const int rows = kv.n_seqs * n_head, join = !parts ? 0 : many ? rows : (rows + kWaves - 1) / kWaves;
   const int account = mass ? kv.n_seqs * kv.Hkv * slices : 0;

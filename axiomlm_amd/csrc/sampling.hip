@@ -274,8 +274,9 @@ struct Weight {
     const double r = y - (near - 6755399441055744.0);
     constexpr double a = 0.6931471805599453 / kTable;
     const double q = fma(fma(fma(r, a * a * a / 6, a * a / 2), r, a), r, 1.0);
-    const uint64_t t = __builtin_bit_cast(uint64_t, table[i & (kTable - 1)]) + ((uint64_t)((uint32_t)(i & -kTable) * ((1u << 20) / kTable)) << 32);
-    return __builtin_bit_cast(uint64_t, fma(q, __builtin_bit_cast(double, t), 4503599627370496.0)) - 0x4330000000000000ull;
+    const uint64_t octaves = (uint64_t)((uint32_t)(i & -kTable) * ((1u << 20) / kTable)) << 32;
+    const double t = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, table[i & (kTable - 1)]) + octaves);
+    return __builtin_bit_cast(uint64_t, fma(q, t, 4503599627370496.0)) - 0x4330000000000000ull;
   }
 };
 __device__ __forceinline__ void fill_table(Lds& s, int shift) {
