@@ -18,6 +18,7 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 2048;
 constexpr float kBinsPerUnit = 64.f;
 constexpr int kList = 2048;  // candidates in LDS
+constexpr int kCounted = 256;  // candidates that are put in order by counting
 constexpr int kAhead = 2;    // loads of a wave under way
 constexpr int kSums = 2048;  // entries of the running sum
 constexpr int kTable = 512;  // entries of the table of 2^(j / kTable)
@@ -103,7 +104,7 @@ struct Lds {
   uint64_t red[2][kWaves];
   uint64_t total, before;
   int n, bin, where;
-  int small[64];
+  int place[kCounted];
 };
 
 // Sum over the workgroup, the same in every thread.  turn: 0 and 1 in turn, so that one barrier is enough.
@@ -161,22 +162,22 @@ __device__ __forceinline__ uint64_t block_max(uint64_t v, Lds& s, int& turn) {
 // s.list[0, n) into descending order (n <= kList); all threads, and a barrier at the end.
 __device__ __forceinline__ void sort_list(Lds& s, int n) {
   __syncthreads();
-  if (n <= 64) {  // places by counting: lane i's candidate against four others in every wave
-    const int i = threadIdx.x & 63, j0 = (threadIdx.x >> 6) * 4;
-    if (threadIdx.x < 64) s.small[i] = 0;
+  int size = 64;
+  while (size < n) size *= 2;
+  if (size <= kCounted) {  // places by counting: each candidate against size^2 / kThreads others in every part of the threads
+    const int i = threadIdx.x & (size - 1), each = size * size / kThreads, j0 = threadIdx.x / size * each;
+    if ((int)threadIdx.x < size) s.place[i] = 0;
     const uint64_t mine = i < n ? s.list[i] : 0;
     int over = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) over += j0 + j < n && s.list[j0 + j] > mine;
+#pragma unroll 4
+    for (int j = j0; j < min(j0 + each, n); ++j) over += s.list[j] > mine;
     __syncthreads();
-    if (over) atomicAdd(&s.small[i], over);
+    if (over) atomicAdd(&s.place[i], over);
     __syncthreads();
-    if (threadIdx.x < 64 && i < n) s.list[s.small[i]] = mine;
+    if ((int)threadIdx.x < n) s.list[s.place[i]] = mine;
     __syncthreads();
     return;
   }
-  int size = 128;
-  while (size < n) size *= 2;
   for (int i = n + threadIdx.x; i < size; i += kThreads) s.list[i] = 0;  // less than every candidate
   __syncthreads();
   for (int k = 2; k <= size; k *= 2)  // bitonic
@@ -310,6 +311,43 @@ __device__ __forceinline__ void sum_tiles(const Row<DT>& row, Lds& s, int group,
     }
   });
   __syncthreads();
+}
+
+// This lane's share of a tile's weights where few logits are kept: the wave queues those in LDS (where s.list was) and
+// weighs them side by side, not every logit that is next to one (us, all weighed / queued: 48.7 / 46.7 for 64 rows of
+// 128000 with top-p).  keep(j): whether z[j] is; of(z): its weight.
+typedef float __attribute__((may_alias)) lds_float;
+template <int E, typename K, typename W>
+__device__ __forceinline__ uint64_t kept_sum(const Weight& weight, const float (&z)[E], Lds& s, const K& keep, const W& of) {
+  constexpr int kRoom = kList * 2 / kWaves;  // logits of a wave's queue
+  lds_float* queue = reinterpret_cast<lds_float*>(s.list) + (threadIdx.x >> 6) * kRoom;
+  const int lane = threadIdx.x & 63;
+  uint64_t mask[E], sum = 0;
+  int n = 0;
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    mask[j] = __builtin_amdgcn_ballot_w64(keep(j));
+    n += __builtin_popcountll(mask[j]);
+  }
+  if (n > kRoom) {
+    uint64_t w[E];
+    weights_of(weight, z, w);
+#pragma unroll
+    for (int j = 0; j < E; ++j) sum += keep(j) ? of(w[j]) : 0;
+    return sum;
+  }
+  int at = 0;
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    if (mask[j] >> lane & 1)
+      queue[at + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask[j], 0u))] =
+          z[j];
+    at += __builtin_popcountll(mask[j]);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  for (int i = lane; i < n; i += 64) sum += of(weight(queue[i]));
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  return sum;
 }
 
 // The first logit, in index order, at which the running sum of weights (s.sums, and f within a group) passes `target`
@@ -447,8 +485,7 @@ __device__ __forceinline__ void deal_slice(Row<DT>& row, int slice, int slices) 
 // with the cut, sums its tiles' weights before that bin and lists the bin's candidates; third: one workgroup a row cuts
 // the list, adds what stays to the sums and picks the token.  Rows whose largest logit is infinite or passes 2^16 or 2^20
 // octaves, and those that list too many, are left to the third launch, which then does everything.  64 rows of 128000
-// with top-p: 15, 19 and 13 us, most of it the weights' 64-bit arithmetic (8 and 11 us; listing the kept logits first and
-// weighing those alone is slower: nuclei of thousands of tokens overflow the list).
+// with top-p: 16, 17 and 11 us; the histogram's pass takes 8, with its additions or without.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t grid_of(float z) {  // 1.5 2^23: the nearest integer in the low bits
   return __builtin_bit_cast(uint32_t, fmaf(z, kBinsPerUnit, 12582912.f));
@@ -580,17 +617,16 @@ __global__ void __launch_bounds__(kThreads) sample_sums_kernel(SampleParams p) {
   uint64_t* list = p.lists + (int64_t)blockIdx.x * kList;
   const int group = tile_group(row.vectors);
   sum_tiles<DT>(row, s, group, [&](int tile, const float (&z)[E], auto add) {
-    uint64_t w[E];
-    weights_of(weight, z, w);
+    int b[E];
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-      const int b = grid_bin(top_grid, z[j]);
-      add(j, (z[j] > -INFINITY) & (b < bin) & (w[j] >= least) ? w[j] : 0);
-      if (b == bin && z[j] > -INFINITY) {
+      b[j] = z[j] > -INFINITY ? grid_bin(top_grid, z[j]) : kBins + 1;
+      if (b[j] == bin) {
         const int at = atomicAdd(&s.n, 1);
         if (at < kList) list[at] = candidate(z[j], row.index(tile, j));
       }
     }
+    add(0, kept_sum(weight, z, s, [&](int j) { return b[j] < bin; }, [&](uint64_t w) { return w >= least ? w : 0; }));
   });
   if (threadIdx.x == 0) p.tops[blockIdx.x].listed = s.n;
   const int tiles = (row.vectors + 63) / 64, groups = (tiles + group - 1) / group;
@@ -980,16 +1016,21 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(SampleParams p) {
   }
 
   // ---- the token ----
-  find_in_order<DT>(row, s, turn, [&](int tile, const float (&z)[E], auto add) {
-    bool any = false;
-#pragma unroll
-    for (int j = 0; j < E; ++j) any |= z[j] >= cut_z;
-    if (!__builtin_amdgcn_ballot_w64(any)) return;
+  const int group = tile_group(row.vectors);
+  auto stayed = [&](uint64_t w) { return stays(w) ? w : 0; };
+  auto weights = [&](int tile, const float (&z)[E], auto add) {
     uint64_t w[E];
     weights_of(weight, z, w);
 #pragma unroll
-    for (int j = 0; j < E; ++j) add(j, kept(z[j], tile, j) & stays(w[j]) ? w[j] : 0);
-  }, u, 0.0);
+    for (int j = 0; j < E; ++j) add(j, kept(z[j], tile, j) ? stayed(w[j]) : 0);
+  };
+  if (cut_z > -INFINITY)
+    sum_tiles<DT>(row, s, group, [&](int tile, const float (&z)[E], auto add) {
+      add(0, kept_sum(weight, z, s, [&](int j) { return kept(z[j], tile, j); }, stayed));
+    });
+  else
+    sum_tiles<DT>(row, s, group, weights);
+  pick_in_order<DT>(row, s, turn, group, weights, u, 0.0);
   if (threadIdx.x == 0) answer(s.where, (float)((double)s.before / (double)s.total));
 }
 

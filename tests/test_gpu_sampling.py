@@ -126,6 +126,13 @@ def test_ties(dev, dtype):
             check(z, u, *s)
 
 
+@pytest.mark.parametrize("k", [63, 64, 65, 100, 128, 129, 255, 256, 257, 500, 1024, 1025, 2047, 2049])
+def test_lists_of_all_lengths(dev, k):
+    z, u = make_logits(dev, 6, 5003, torch.float32, 14)
+    check(z, u, 1.5, k, 0.95, 0.0)
+    check((z * 8).round() / 8, u, 2.0, k, 1.0, 0.0)  # ties at the border
+
+
 def test_top_k_past_32_bits_is_no_filter(dev):
     z, u = make_logits(dev, 3, 500, torch.float16, 12)
     want = K.sample_tokens(z, u)
