@@ -1040,7 +1040,7 @@ namespace {
 
 // Workgroups that share a row, 8192 logits or more each: none where rows or vocabulary are too small for the three
 // launches to pay, or where top-k leaves rows a list that one workgroup is as fast with.  us, one workgroup a row / split:
-// with top-p 64 rows of 128000 93 / 51 (four slices), 100 of 50000 47 / 42 (two), 20 of 40000 36 / 32 (four), but 8 of
+// with top-p 64 rows of 128000 93 / 44 (four slices), 100 of 50000 47 / 42 (two), 20 of 40000 36 / 32 (four), but 8 of
 // 30000 30 / 31 (three); without one row of 100000 42 / 21 (twelve), 60 of 50000 23 / 22 and in fp32 28 / 23 (four), but
 // 20 of 40000 19 / 21 (four) and 100 of 50000 23 / 26 (two); 60 of 20000 with top-k in most 26 / 45 (two).
 int slices_of(int rows, int V, bool top_k, bool top_p) {
